@@ -10,21 +10,17 @@
 namespace thk {
 
 // Development timeline (libthk_trace.so only, built with -DTHK_TRACE; tools/step_trace.py): every wave stamps the 100 MHz
-// s_memrealtime counter at up to four points of its kernel into [workgroup][wave (8)][4].  Scalar instructions only (the stamp
-// is written with s_store_dwordx2, flushed by s_dcache_wb at the last one): no VGPR, no exec-mask branch, so the register
-// allocation and occupancy of the traced build stay those of the product build.  In the product build the macro is empty.
+// s_memrealtime counter at up to four points of its kernel into [workgroup][wave (8)][4].  The counter is read by a scalar
+// instruction and written by lane 0 with an ordinary vector store.  In the product build the macro is empty.
 #ifdef THK_TRACE
 __device__ __forceinline__ void thk_stamp(unsigned long long* tr, int bid, int slot) {
     if (tr) {                                                            // kernel argument: a scalar branch
         unsigned long long t;
         asm volatile("s_memrealtime %0\n\ts_waitcnt lgkmcnt(0)" : "=s"(t));
-        const unsigned off = __builtin_amdgcn_readfirstlane(((unsigned)bid * 8u + (threadIdx.x >> 6)) * 32u + (unsigned)slot * 8u);
-        asm volatile("s_store_dwordx2 %0, %1, %2" ::"s"(t), "s"(tr), "s"(off));
-        if (slot == 3) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb" ::: "memory");
+        if ((threadIdx.x & 63) == 0) tr[((size_t)bid * 8u + (threadIdx.x >> 6)) * 4u + slot] = t;
     }
 }
-// THK_TRACE=1 stamps kernel entry and exit only (register allocation identical to the product build, checked with
-// -Rpass-analysis=kernel-resource-usage); THK_TRACE=2 adds the two inner stamps, which cost the mat-vec kernels 20+ VGPRs.
+// THK_TRACE=1 stamps kernel entry and exit only; THK_TRACE=2 adds the two inner stamps, which cost the mat-vec kernels 20+ VGPRs.
 #define THK_STAMP(tr, bid, slot) do { if (THK_TRACE >= 2 || (slot) == 0 || (slot) == 3) thk_stamp((tr), (bid), (slot)); } while (0)
 #else
 #define THK_STAMP(tr, bid, slot) do { } while (0)
