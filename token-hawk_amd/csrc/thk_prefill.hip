@@ -904,6 +904,22 @@ __global__ __launch_bounds__(256) void reduce_store_kernel(const float* __restri
     if (mode == 1) s = *dst + s;
     *dst = s;
 }
+// The f16 hi and lo parts of a * b: hi is the product rounded to f32 and then to f16, lo the rest of the exact product.  The empty asm pins
+// both f32 values: left alone, the compiler rounds the exact product to f16 in one step for the remainder but in two for the stored hi,
+// and where the two differ hi + lo misses the product by a step of hi.
+struct HiLo { _Float16 hi, lo; };
+__device__ __forceinline__ HiLo split_product(float a, float b) {
+    float v = a * b;
+    asm("" : "+v"(v));
+    const _Float16 hi = (_Float16)v;
+    float r = fmaf(a, b, -(float)hi);
+    asm("" : "+v"(r));
+    return {hi, (_Float16)r};
+}
+__device__ __forceinline__ float square_rounded(float x) {      // not contracted into the sum it goes to
+#pragma clang fp contract(off)
+    return x * x;
+}
 // x = X + sum (residual, K11) -> X, and straight on to the NEXT GEMM's operand: the hi/lo image of x * gain (deferred norm, see
 // ximg_from_rows_kernel) and this workgroup's share of every token's sum of squares.  A workgroup = 256 consecutive q = one
 // (token tile, 32-row fragment): 32 tokens x 8 threads, each with 4 rows.  Replaces reduce_store + norm -> image (two launches).
@@ -927,9 +943,9 @@ __global__ __launch_bounds__(256) void reduce_resid_ximg_kernel(const float* __r
         const float sc = ssq_pow2(ssq_scale, tok, p.R);          // power of two near this token's 1/rms (from its previous norm input)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float v = (x[e] * sc) * g[e];
-            hi[e] = (_Float16)v; lo[e] = (_Float16)(v - (float)hi[e]);
-            ss += x[e] * x[e];
+            const HiLo v = split_product(x[e] * sc, g[e]);
+            hi[e] = v.hi; lo[e] = v.lo;
+            ss += square_rounded(x[e]);
         }
     }
     if (r < p.R) {                                  // pad tokens of the image are zeros
@@ -994,8 +1010,9 @@ __global__ __launch_bounds__(256) void reduce_swiglu_ximg_kernel(const float* __
         if (ssq) { const float inv = ssq_inv(ssq, tok, p.C) / ssq_pow2(ssq_scale, tok, p.C); u1 = u1 * inv; u3 = u3 * inv; }    // deferred norm
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float sl = u1[e] / (1.0f + expf(-u1[e])), v = sl * u3[e];
-            hi[e] = (_Float16)v; lo[e] = (_Float16)(v - (float)hi[e]);
+            const float sl = u1[e] / (1.0f + expf(-u1[e]));
+            const HiLo v = split_product(sl, u3[e]);
+            hi[e] = v.hi; lo[e] = v.lo;
         }
     }
     const size_t sub = (size_t)(r & 4) * 2;                              // second half of the piece
