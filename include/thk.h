@@ -354,6 +354,45 @@ int thk_peer_check(thk_peer* p);                         /* THK_ERR_STATE once a
 int thk_peer_memory_kind(const thk_peer* p);             /* THK_PEER_MEM_* of this stage's mailbox */
 int thk_peer_destroy(thk_peer* p);
 
+/* ---------------------------------------------------------------- 8-bit K/V cache
+ * One layer's K/V cache of one sequence, held as 8-bit codes with a scale for every block of THK_KV8_BLOCK positions and K/V head: a quarter
+ * of the f32 cache's bytes (thk_kv_append / thk_attn_decode / thk_attn_prefill), attention that reads the codes, and eviction by the
+ * attention weight a position has drawn.  The reference keeps an f32 cache and ends when it is full (th-llama-loader.cpp:335).
+ *   block   positions [16 b, 16 b + 16) of one K/V head; amax = the largest magnitude in its rows (the positions appended so far)
+ *   scale   f32(amax / 127);  code = rint(x * f32(127 / amax)), the exact product rounded once, ties to even;  value = f32(code * scale)
+ *           amax < 2^-100: the block is zero.  A NaN or an infinity in a block makes its scale NaN: rows that may see one of its positions
+ *           get NaN, others do not (K: through the score; V: in the output only, the weights stay).
+ *   grouped heads: query head h reads K/V head h / (H / H_kv).
+ * The cache does not count positions: the caller passes them, as for thk_kv_append, and has appended [0, T) before it attends to T.  Calls are
+ * stream-ordered, allocate nothing and may be captured into a graph (create and destroy may not); a replay uses the captured positions and
+ * pointers.  The cache owns the workspace of its calls: calls and replays of ONE cache must not overlap on two streams.
+ * All pointers are 16-byte aligned dev pointers; weight arrays ("mass") are f32 [H_kv][n_ctx of their cache], only the entries named are touched. */
+typedef struct thk_kv8 thk_kv8;
+#define THK_KV8_BLOCK 16
+/* n_ctx 1 .. 2^26, H a multiple of H_kv (<= 1024), D 64 | 128 | 256.  Destroy before its context. */
+int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_kv, int64_t D, thk_kv8** out);
+int thk_kv8_destroy(thk_kv8* kv);
+int64_t thk_kv8_bytes(const thk_kv8* kv);   /* device memory the cache holds, workspace included */
+int64_t thk_kv8_n_ctx(const thk_kv8* kv);
+/* Positions [pos, pos + n_tok) from k, v [n_tok, H_kv, D] (thk_kv_append's rows).  A block that is still open is quantised anew from its
+ * unrounded rows, so n_tok tokens at once and one by one leave the same bits.  Appending before the end truncates: the later positions of
+ * the last block touched are cleared, and if that block is not the one appended to last, its earlier rows enter as the values they had. */
+int thk_kv8_append(thk_kv8* kv, const float* k, const float* v, int64_t pos, int64_t n_tok);
+/* The values of positions [pos, pos + n_tok): f32 [n_tok, H_kv, D]; either output may be NULL. */
+int thk_kv8_read(thk_kv8* kv, int64_t pos, int64_t n_tok, float* k_out, float* v_out);
+/* thk_attn_decode over the first T positions: q and out are [H, D].  With mass_in / mass_out (both or neither, may be the same array):
+ * mass_out[j][t] = mass_in[j][t] + the softmax weights of K/V head j's query heads on position t, t < T. */
+int thk_kv8_attn_decode(thk_kv8* kv, const float* q, int64_t T, const float* mass_in, float* mass_out, float* out);
+/* thk_attn_prefill: M rows, row i sees positions <= n_past + i (appended before); q and out are [M, H, D].  The weights are summed over rows too. */
+int thk_kv8_attn_prefill(thk_kv8* kv, const float* q, int64_t n_past, int64_t M, const float* mass_in, float* mass_out, float* out);
+/* Keeps n_keep of src's first T positions, for every K/V head its own: the first n_sink, the last n_recent and the heaviest of the others by
+ * mass_in (ties: the lower position; NaN counts as lightest), in order, as positions [0, n_keep) of dst - another cache of the same context,
+ * K/V heads and head dim.  kept (dev int32 [H_kv][n_keep]) receives the positions, mass_out (may be NULL) their weights.  Sixteen kept
+ * positions that were one block keep their codes; other blocks are quantised anew from the values.  Keys keep the rotation of the position
+ * they were appended at.  src is left as it is: a ring of caches needs one spare, whatever the number of layers. */
+int thk_kv8_evict(thk_kv8* src, int64_t T, int64_t n_keep, int64_t n_sink, int64_t n_recent, const float* mass_in, thk_kv8* dst, float* mass_out,
+                  int32_t* kept);
+
 /* Tuning knobs (integers, by name) so the bench can sweep launch geometry without
  * rebuilding.  Decode knobs must be set before thk_model_finalize; prefill knobs are read
  * per call.  Unknown names return THK_ERR_NOTFOUND.

@@ -19,7 +19,7 @@ from . import _capi
 from ._capi import (HParams, THK_F16, THK_F32, THK_LMHEAD_CORRECT, THK_LMHEAD_FAITHFUL, THK_OK, THK_STAGE_EMBED,
                     THK_STAGE_HEAD)
 
-__all__ = ["Context", "Buffer", "Model", "ModelShape", "ThkError", "LLAMA_7B", "LLAMA_13B", "TINY", "TINY_Q1",
+__all__ = ["Context", "Buffer", "KvCache8", "Model", "ModelShape", "ThkError", "LLAMA_7B", "LLAMA_13B", "TINY", "TINY_Q1",
            "THK_LMHEAD_CORRECT", "THK_LMHEAD_FAITHFUL", "THK_STAGE_EMBED", "THK_STAGE_HEAD", "TENSOR_SEED", "TENSOR_SIGMA"]
 
 TENSOR_SEED = 20230517   # synthetic-weight key
@@ -230,6 +230,53 @@ class Buffer:
             self.free()
         except Exception:
             pass
+
+
+class KvCache8:
+    """thk_kv8: one layer's K/V cache in 8-bit codes with a scale per block of 16 positions and K/V head (pointers are device pointers / Buffers)."""
+
+    BLOCK = 16
+
+    def __init__(self, ctx: Context, n_ctx: int, n_head: int, n_head_kv: int, head_dim: int):
+        self.ctx, self.n_ctx, self.n_head, self.n_head_kv, self.head_dim = ctx, n_ctx, n_head, n_head_kv, head_dim
+        h = C.c_void_p()
+        ctx.check(ctx.lib.thk_kv8_create(ctx.h, n_ctx, n_head, n_head_kv, head_dim, C.byref(h)), "thk_kv8_create")
+        self.h = h
+
+    def close(self):
+        if getattr(self, "h", None) and getattr(self.ctx, "h", None):
+            self.ctx.check(self.ctx.lib.thk_kv8_destroy(self.h), "thk_kv8_destroy")
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def nbytes(self) -> int:
+        return int(self.ctx.lib.thk_kv8_bytes(self.h))
+
+    def append(self, k, v, pos: int, n_tok: int):
+        """Positions [pos, pos + n_tok) from k, v f32 [n_tok, n_head_kv, head_dim]."""
+        self.ctx.check(self.ctx.lib.thk_kv8_append(self.h, _ptr(k), _ptr(v), pos, n_tok), "thk_kv8_append")
+
+    def read(self, pos: int, n_tok: int, k_out, v_out):
+        """The values of positions [pos, pos + n_tok) as f32 [n_tok, n_head_kv, head_dim]; either output may be None."""
+        self.ctx.check(self.ctx.lib.thk_kv8_read(self.h, pos, n_tok, _ptr(k_out), _ptr(v_out)), "thk_kv8_read")
+
+    def attn_decode(self, q, T: int, out, mass_in=None, mass_out=None):
+        """One query token over the first T positions; mass_out = mass_in + its softmax weights (f32 [n_head_kv, n_ctx])."""
+        self.ctx.check(self.ctx.lib.thk_kv8_attn_decode(self.h, _ptr(q), T, _ptr(mass_in), _ptr(mass_out), _ptr(out)), "thk_kv8_attn_decode")
+
+    def attn_prefill(self, q, n_past: int, M: int, out, mass_in=None, mass_out=None):
+        """M query rows, row i over positions <= n_past + i."""
+        self.ctx.check(self.ctx.lib.thk_kv8_attn_prefill(self.h, _ptr(q), n_past, M, _ptr(mass_in), _ptr(mass_out), _ptr(out)), "thk_kv8_attn_prefill")
+
+    def evict(self, dst: "KvCache8", T: int, n_keep: int, n_sink: int, n_recent: int, mass_in, mass_out, kept):
+        """Every K/V head's n_keep positions (first n_sink, last n_recent, heaviest others) into dst; kept: dev int32 [n_head_kv, n_keep]."""
+        self.ctx.check(self.ctx.lib.thk_kv8_evict(self.h, T, n_keep, n_sink, n_recent, _ptr(mass_in), dst.h, _ptr(mass_out), _ptr(kept)), "thk_kv8_evict")
 
 
 class Model:

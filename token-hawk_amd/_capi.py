@@ -122,6 +122,15 @@ SIGNATURES = {
     "thk_peer_check": (C.c_int, [vp]),
     "thk_peer_memory_kind": (C.c_int, [vp]),
     "thk_peer_destroy": (C.c_int, [vp]),
+    "thk_kv8_create": (C.c_int, [vp, i64, i64, i64, i64, pp]),
+    "thk_kv8_destroy": (C.c_int, [vp]),
+    "thk_kv8_bytes": (i64, [vp]),
+    "thk_kv8_n_ctx": (i64, [vp]),
+    "thk_kv8_append": (C.c_int, [vp, vp, vp, i64, i64]),
+    "thk_kv8_read": (C.c_int, [vp, i64, i64, vp, vp]),
+    "thk_kv8_attn_decode": (C.c_int, [vp, vp, i64, vp, vp, vp]),
+    "thk_kv8_attn_prefill": (C.c_int, [vp, vp, i64, i64, vp, vp, vp]),
+    "thk_kv8_evict": (C.c_int, [vp, i64, i64, i64, i64, vp, vp, vp, vp]),
     "thk_set_tunable": (C.c_int, [vp, C.c_char_p, i64]),
     "thk_get_tunable": (C.c_int, [vp, C.c_char_p, C.POINTER(i64)]),
 }

@@ -1,0 +1,47 @@
+// thk_kv8.hpp — the 8-bit K/V cache (thk_kv8_* of include/thk.h): device layout and launchers.  Internal.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace thk {
+
+static const int kKv8Block = 16;      // positions that share one K scale and one V scale per K/V head
+static const int kKv8Tile = 64;       // positions one step of the attention kernels takes: the cache is padded to whole tiles
+static const int kKv8RowSlab = 2048;  // prompt rows one attention launch takes (sizes the per-row statistics)
+
+// Device memory of one cache.  n_blk = blocks per head, a multiple of 4 (whole tiles).
+//   k    int8 [Hkv][n_blk][16][D]    codes, row-major: a position's D codes are contiguous
+//   v    int8 [Hkv][n_blk][D][16]    codes, transposed inside the block: the 16 positions of one dimension are contiguous, which is
+//                                    the operand chunk of one lane when positions are the summed axis of a matrix instruction
+//   ks, vs f32 [Hkv][n_blk]          scales
+//   tail f32 [2][Hkv][16][D]         the rows of the block that was appended to last, unrounded (K, then V)
+//   tail_at int2 [2][Hkv]            which block that is (-1: none) and how many of its rows tail holds
+struct Kv8View {
+    int8_t *k, *v;
+    float *ks, *vs;
+    float* tail;
+    int2* tail_at;
+    int n_blk, H, Hkv, D;
+};
+
+struct Kv8Attn {
+    Kv8View c;
+    const float* q;                   // [M][H][D]
+    float* out;                       // [M][H][D]
+    int n_past, M;                    // row i sees positions <= n_past + i
+    float2* ml;                       // [M][H] running maximum (base-2 scores) and sum of every row, for the weight count; or null
+    const float* mass_in;             // [Hkv][mass_ld] or null (then no weights are counted)
+    float* mass_out;
+    int64_t mass_ld;
+    int mass_n;                       // entries per head that are written: all positions of the call, also those this slab's rows do not see yet
+};
+
+hipError_t launch_kv8_append(const Kv8View& c, const float* k, const float* v, int64_t pos, int64_t n, hipStream_t st);
+hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_out, float* v_out, hipStream_t st);
+hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recent, const float* mass_in, int64_t ld_in, float* mass_out, int64_t ld_out, int32_t* kept,
+                             hipStream_t st);
+hipError_t launch_kv8_move(const Kv8View& src, const Kv8View& dst, int n_keep, const int32_t* kept, hipStream_t st);
+hipError_t launch_kv8_attn_rows(const Kv8Attn& a, hipStream_t st);
+hipError_t launch_kv8_attn_mass(const Kv8Attn& a, hipStream_t st);
+
+}  // namespace thk
