@@ -84,9 +84,9 @@ def test_create_failures(env, lib):
 
 def test_size_of_a_cache(env, lib):
     """A quarter of the f32 cache, and little beside it."""
-    h = env.create(4096, 32, 32, 128)
-    codes = 2 * 32 * 4096 * 128
-    assert codes < lib.thk_kv8_bytes(h) < codes * 1.15 and lib.thk_kv8_n_ctx(h) == 4096
+    h = env.create(16384, 32, 32, 128)
+    codes = 2 * 32 * 16384 * 128
+    assert codes < lib.thk_kv8_bytes(h) < codes * 1.07 and lib.thk_kv8_n_ctx(h) == 16384
     assert lib.thk_kv8_destroy(h) == 0
 
 

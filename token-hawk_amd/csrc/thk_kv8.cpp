@@ -10,6 +10,9 @@ struct thk_kv8 {
     void* mem = nullptr;        // one allocation: codes, scales, tail rows
     size_t mem_bytes = 0;
     float2* ml = nullptr;       // per-row softmax statistics of an attention call that counts weights
+    float* part_o = nullptr;    // parts of rows that are split over the positions
+    float2* part_ml = nullptr;
+    float* scores = nullptr;    // [H][padded n_ctx]: a single row's scores, for the weight count
 };
 
 namespace {
@@ -53,7 +56,8 @@ extern "C" int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_
     v.H = (int)H; v.Hkv = (int)H_kv; v.D = (int)D;
     const size_t codes = (size_t)H_kv * v.n_blk * kKv8Block * D, scales = up256((size_t)H_kv * v.n_blk * 4), tail = (size_t)2 * H_kv * kKv8Block * D * 4;
     const size_t at = up256((size_t)2 * H_kv * sizeof(int2)), ml = (size_t)kKv8RowSlab * H * sizeof(float2);
-    kv->mem_bytes = 2 * codes + 2 * scales + tail + at + ml;
+    const size_t part = (size_t)kKv8SplitRows * (D * 4 + sizeof(float2)), scores_bytes = (size_t)H * v.n_blk * kKv8Block * 4;
+    kv->mem_bytes = 2 * codes + 2 * scales + tail + at + ml + part + scores_bytes;
     hipError_t e = hipMalloc(&kv->mem, kv->mem_bytes);
     if (e != hipSuccess) {
         (void)hipGetLastError();
@@ -68,7 +72,10 @@ extern "C" int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_
     v.vs = (float*)p; p += scales;
     v.tail = (float*)p; p += tail;
     v.tail_at = (int2*)p; p += at;
-    kv->ml = (float2*)p;
+    kv->ml = (float2*)p; p += ml;
+    kv->part_o = (float*)p; p += (size_t)kKv8SplitRows * D * 4;
+    kv->part_ml = (float2*)p; p += (size_t)kKv8SplitRows * sizeof(float2);
+    kv->scores = (float*)p;
     e = hipMemsetAsync(kv->mem, 0, kv->mem_bytes, ctx->stream);
     if (e == hipSuccess) e = hipMemsetAsync(v.tail_at, 0xFF, (size_t)2 * H_kv * sizeof(int2), ctx->stream);     // no block is open
     if (e != hipSuccess) {
@@ -131,8 +138,18 @@ static int kv8_attention(thk_kv8* kv, const char* what, const float* q, int64_t 
         a.c = kv->view; a.q = q + i * row; a.out = out + i * row;
         a.n_past = (int)(n_past + i); a.M = (int)(M - i < kKv8RowSlab ? M - i : kKv8RowSlab);
         if (mass_out) { a.ml = kv->ml; a.mass_in = mass_in; a.mass_out = mass_out; a.mass_ld = kv->n_ctx; a.mass_n = (int)(n_past + M); }
-        HIPCHK(ctx, launch_kv8_attn_rows(a, ctx->stream));
-        if (mass_out) HIPCHK(ctx, launch_kv8_attn_mass(a, ctx->stream));
+        const int64_t groups = ((int64_t)a.M * (a.c.H / a.c.Hkv) + 15) / 16 * a.c.Hkv;      // workgroups without a split
+        if (groups <= 1024) {
+            Kv8Split sp{};
+            const int64_t tiles = (a.n_past + a.M + kKv8Tile - 1) / kKv8Tile, most = (tiles + 3) / 4;
+            int64_t n = 512 / groups;
+            if (n > most) n = most;
+            if (n > kKv8SplitRows / ((int64_t)a.M * a.c.H)) n = kKv8SplitRows / ((int64_t)a.M * a.c.H);
+            sp.n = n < 1 ? 1 : (int)n; sp.part_o = kv->part_o; sp.part_ml = kv->part_ml;
+            if (mass_out && a.M == 1) { sp.scores = kv->scores; sp.scores_ld = (int64_t)a.c.n_blk * kKv8Block; }
+            HIPCHK(ctx, launch_kv8_attn_split(a, sp, ctx->stream));
+        } else HIPCHK(ctx, launch_kv8_attn_rows(a, ctx->stream));
+        if (mass_out && a.M > 1) HIPCHK(ctx, launch_kv8_attn_mass(a, ctx->stream));
         mass_in = mass_out;
     }
     return THK_OK;

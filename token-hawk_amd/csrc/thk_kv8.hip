@@ -311,6 +311,270 @@ __global__ __launch_bounds__(256) void kv8_attn_mass_kernel(Kv8Attn a, float sca
     if ((tid & 15) == 0 && t < a.mass_n) a.mass_out[(size_t)hkv * a.mass_ld + t] = a.mass_in[(size_t)hkv * a.mass_ld + t] + sum;
 }
 
+
+// ---------------------------------------------------------------- attention of few rows: i8 matrix instructions, split over the positions
+// out_n = sum_t p_nt v_t with p = softmax(q_n . k_t), for up to 16 (row, head) columns n that read one K/V head.  Both products run on
+// v_mfma_i32_16x16x64_i8 with the cache's codes as they are - no conversion - and the f32 operand (q, then the weights) as a fixed-point
+// number of three balanced base-256 digits: x = d2 2^16 + d1 2^8 + d0, each digit an i8 operand of its own product, the three i32 sums
+// exact.  q is fixed relative to its column's largest entry (23 bits), the weights p * v_scale relative to the largest of their column
+// in the tile of 64 positions (a power of two, 21 to 22 bits): errors stay at f32's own.
+// Operand layout (A: row = lane % 16, B: column = lane % 16, both 16 consecutive k per lane of chunk lane / 16; result: column lane % 16,
+// rows 4 (lane / 16) + i).  The k order is free as long as A and B share it, and the row order of the first product is chosen so that
+// lane chunk c ends up with the scores of the 16 positions of block c: then one K scale and one V scale per lane serve a whole tile, and
+// the second product's B operand is what the lane already holds - no exchange between lanes.
+typedef int i4 __attribute__((ext_vector_type(4)));
+struct U2 { unsigned a, b; };
+// Between them, a and b hold a value and that of the lane 16 (32) away, in every lane.  The swap works on two registers: the empty asm keeps
+// the compiler from giving it the same one twice, which would leave the value where it is.
+__device__ __forceinline__ U2 pair16(unsigned v) {
+    unsigned w = v;
+    asm("" : "+v"(w));
+    const auto r = __builtin_amdgcn_permlane16_swap(v, w, false, false);
+    return {r[0], r[1]};
+}
+__device__ __forceinline__ U2 pair32(unsigned v) {
+    unsigned w = v;
+    asm("" : "+v"(w));
+    const auto r = __builtin_amdgcn_permlane32_swap(v, w, false, false);
+    return {r[0], r[1]};
+}
+__device__ __forceinline__ float as_f(unsigned v) { return __builtin_bit_cast(float, v); }
+__device__ __forceinline__ unsigned as_u(float v) { return __builtin_bit_cast(unsigned, v); }
+// over the four lanes of a column
+__device__ __forceinline__ float chunks_max(float v) {
+    U2 r = pair16(as_u(v));
+    r = pair32(as_u(fmaxf(as_f(r.a), as_f(r.b))));
+    return fmaxf(as_f(r.a), as_f(r.b));
+}
+__device__ __forceinline__ unsigned chunks_max_bits(unsigned v) {
+    U2 r = pair16(v);
+    r = pair32(r.a > r.b ? r.a : r.b);
+    return r.a > r.b ? r.a : r.b;
+}
+__device__ __forceinline__ float chunks_sum(float v) {
+    U2 r = pair16(as_u(v));
+    r = pair32(as_u(as_f(r.a) + as_f(r.b)));
+    return as_f(r.a) + as_f(r.b);
+}
+// Four numbers given as x + 0x808080 (x = d2 2^16 + d1 2^8 + d0, the low three bytes are the digits plus 128): their digits, four to a word.
+__device__ __forceinline__ void pack_digits(unsigned e0, unsigned e1, unsigned e2, unsigned e3, int& d2, int& d1, int& d0) {
+    const unsigned a = __builtin_amdgcn_perm(e1, e0, 0x05040100u), b = __builtin_amdgcn_perm(e3, e2, 0x05040100u);     // bytes: e0.0 e0.1 e1.0 e1.1
+    const unsigned u = __builtin_amdgcn_perm(e1, e0, 0x0C0C0602u), w = __builtin_amdgcn_perm(e3, e2, 0x06020C0Cu);
+    d0 = (int)(__builtin_amdgcn_perm(b, a, 0x06040200u) ^ 0x80808080u);
+    d1 = (int)(__builtin_amdgcn_perm(b, a, 0x07050301u) ^ 0x80808080u);
+    d2 = (int)((u | w) ^ 0x80808080u);
+}
+__device__ __forceinline__ float join_digits(int i2, int i1, int i0) { return fmaf((float)i2, 65536.f, (float)(i1 * 256 + i0)); }   // |i1| <= 256 * 2^14: no overflow
+
+// The B operand of q: digits of columns n = 16 cg + lane % 16, dimensions (lane / 16) * D/4 + 16 kc + j.  Returns the step of the fixed point.
+template <int D>
+__device__ __forceinline__ float load_q_digits(const float* q, bool valid, i4 (&qd)[3][D / 64]) {
+    float x[D / 4];
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+        const f4 v = valid ? reinterpret_cast<const f4*>(q)[i] : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { x[4 * i + j] = v[j]; const unsigned a = abs_bits(v[j]); m = a > m ? a : m; }
+    }
+    m = chunks_max_bits(m);
+    const float amax = __builtin_bit_cast(float, m);
+    const bool some = amax >= 0x1p-100f;                                   // also false for NaN
+    const float inv = some && m < 0x7F800000u ? 8355000.f / amax : 0.f;    // below 127 (2^16 + 2^8 + 1), the largest sum of three balanced digits, by more than the roundings
+#pragma unroll
+    for (int kc = 0; kc < D / 64; ++kc)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            unsigned e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[j] = (unsigned)((int)rintf(x[16 * kc + 4 * w + j] * inv) + 0x808080);
+            int d2, d1, d0;
+            pack_digits(e[0], e[1], e[2], e[3], d2, d1, d0);
+            qd[2][kc][w] = d2; qd[1][kc][w] = d1; qd[0][kc][w] = d0;
+        }
+    if (m >= 0x7F800000u) return __builtin_bit_cast(float, 0x7FC00000u);    // a query that is not finite: every score is NaN
+    return some ? amax / 8355000.f : 0.f;
+}
+
+template <int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_split_kernel(Kv8Attn a, Kv8Split sp, float scale) {
+    constexpr int KC = D / 64, NG = D / 16;
+    __shared__ float so[4][16][D + 4], sml[4][16][2];
+    const Kv8View& c = a.c;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, ch = lane >> 4;
+    const int split = blockIdx.x, hkv = blockIdx.y, col = blockIdx.z * 16 + n, G = c.H / c.Hkv, cols = a.M * G;
+    const int row = col / G, last_col = min((int)blockIdx.z * 16 + 15, cols - 1);
+    const bool valid = col < cols;
+    const int T = a.n_past + last_col / G + 1, first_lim = a.n_past + (int)blockIdx.z * 16 / G, lim = valid ? a.n_past + row : T - 1;   // positions <= lim are seen
+    const int tiles = (T + kKv8Tile - 1) / kKv8Tile, per = (tiles + sp.n - 1) / sp.n, t1 = min((split + 1) * per, tiles);
+    const size_t orow = valid ? (size_t)row * c.H + hkv * G + col % G : 0;
+
+    const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + 16 * (n >> 2) + (n & 3)) * D + ch * (D / 4);
+    const int8_t* vb = c.v + (((size_t)hkv * c.n_blk + ch) * D + n) * 16;
+    const float *ksb = c.ks + (size_t)hkv * c.n_blk + ch, *vsb = c.vs + (size_t)hkv * c.n_blk + ch;
+    i4 kr[4][KC], vr[NG];
+    float ks = 0.f, vs = 0.f;
+    auto load_k = [&](int t) {
+        const int8_t* p = kb + (size_t)t * (kKv8Tile * D);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) kr[g][kc] = *reinterpret_cast<const i4*>(p + (4 * g) * D + kc * 16);
+        ks = ksb[(size_t)t * 4];
+    };
+    auto load_v = [&](int t) {
+        const int8_t* p = vb + (size_t)t * (kKv8Tile * D);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) vr[g] = *reinterpret_cast<const i4*>(p + g * 256);
+        vs = vsb[(size_t)t * 4];
+    };
+    int t = split * per + w;
+    if (t < t1) { load_k(t); load_v(t); }
+    i4 qd[3][KC];
+    const float qf = load_q_digits<D>(a.q + orow * D + ch * (D / 4), valid, qd) * scale;
+    float m = -INFINITY, l = 0.f;
+    f4 o[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) o[g] = f4{0.f, 0.f, 0.f, 0.f};
+    for (; t < t1; t += 4) {
+        float s[16];
+        const float kf = qf * ks;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            i4 acc[3];
+#pragma unroll
+            for (int d = 0; d < 3; ++d) {
+                acc[d] = i4{0, 0, 0, 0};
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[g][kc], qd[d][kc], acc[d], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * g + i] = join_digits(acc[2][i], acc[1][i], acc[0][i]) * kf;
+            if (g & 1) __builtin_amdgcn_sched_barrier(0);            // two groups in flight: more only cost registers
+        }
+        const int tn = t + 4;
+        if (tn < t1) load_k(tn);
+        const int pos = t * kKv8Tile + ch * 16;
+        if (t * kKv8Tile + kKv8Tile - 1 > first_lim) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = pos + i <= lim ? s[i] : -INFINITY;
+        }
+        if (sp.scores && valid) {
+            f4* ps = reinterpret_cast<f4*>(sp.scores + orow * sp.scores_ld + pos);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) ps[g] = f4{s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+        }
+        float sm = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) sm = fmaxf(sm, s[i]);
+        const float mn = fmaxf(m, chunks_max(sm)), mu = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - mu);
+        float ls = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(s[i] - mu); ls += s[i]; }
+        l = fmaf(l, al, ls);
+        m = mn;
+        // weights p * vs in steps of 2^(e - 22), e the exponent of the tile's largest: whole numbers below 2^22.  Blocks no row of this
+        // column sees (p = 0 throughout) must not bring in their scale, which may be NaN.
+        const float vsu = pos <= lim ? vs : 0.f;
+        const float wm = __builtin_bit_cast(float, chunks_max_bits(__builtin_bit_cast(unsigned, __builtin_amdgcn_exp2f(sm - mu) * vsu)));
+        const int e = __builtin_amdgcn_frexp_expf(wm);
+        const float fac = ldexpf(vsu, 22 - e), f = ldexpf(1.f, e - 22) + (wm - wm);                  // wm - wm: 0, or NaN if wm is not finite
+        i4 pd[3];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            unsigned x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = __builtin_bit_cast(unsigned, fmaf(s[4 * g + i], fac, 8388608.f)) + 0x00808080u;
+            int d2, d1, d0;
+            pack_digits(x[0], x[1], x[2], x[3], d2, d1, d0);
+            pd[2][g] = d2; pd[1][g] = d1; pd[0][g] = d0;
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const i4 z = i4{0, 0, 0, 0};
+            const i4 a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[g], pd[2], z, 0, 0, 0);
+            const i4 a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[g], pd[1], z, 0, 0, 0);
+            const i4 a0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[g], pd[0], z, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[g][i] = fmaf(o[g][i], al, f * join_digits(a2[i], a1[i], a0[i]));
+            if (g & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+        if (tn < t1) load_v(tn);
+    }
+    l = chunks_sum(l);
+    // join the four waves: columns n, dimensions 16 g + 4 ch + i
+    if (valid) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) *reinterpret_cast<f4*>(&so[w][n][16 * g + 4 * ch]) = o[g];
+        if (ch == 0) { sml[w][n][0] = m; sml[w][n][1] = l; }
+    }
+    __syncthreads();
+    const int nv = min(cols - (int)blockIdx.z * 16, 16);
+    for (int j = threadIdx.x; j < nv * (D / 4); j += 256) {
+        const int cn = j / (D / 4), d = (j % (D / 4)) * 4, cc = blockIdx.z * 16 + cn;
+        const size_t r = (size_t)(cc / G) * c.H + hkv * G + cc % G;
+        const float mm = fmaxf(fmaxf(sml[0][cn][0], sml[1][cn][0]), fmaxf(sml[2][cn][0], sml[3][cn][0])), mu = mm == -INFINITY ? 0.f : mm;
+        f4 sum = f4{0.f, 0.f, 0.f, 0.f};
+        float ll = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float e = __builtin_amdgcn_exp2f(sml[i][cn][0] - mu);
+            const f4 v = *reinterpret_cast<const f4*>(&so[i][cn][d]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k] = fmaf(v[k], e, sum[k]);
+            ll = fmaf(sml[i][cn][1], e, ll);
+        }
+        if (sp.n == 1) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k] = sum[k] / ll;
+            *reinterpret_cast<f4*>(a.out + r * D + d) = sum;
+        } else {
+            *reinterpret_cast<f4*>(sp.part_o + (r * sp.n + split) * D + d) = sum;
+        }
+        if (d == 0) {
+            if (sp.n > 1) sp.part_ml[r * sp.n + split] = float2{mm, ll};
+            else if (a.ml) a.ml[r] = float2{mm, ll};
+        }
+    }
+}
+// Joins the splits of a row and head: one workgroup of D / 4 threads each; the statistics go to ml where weights are counted.
+template <int D>
+__global__ __launch_bounds__(64) void kv8_attn_join_kernel(Kv8Attn a, Kv8Split sp) {
+    const size_t r = blockIdx.x;
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < sp.n; i += 64) m = fmaxf(m, sp.part_ml[r * sp.n + i].x);
+    m = wave_max(m);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int i = threadIdx.x; i < sp.n; i += 64) { const float2 t = sp.part_ml[r * sp.n + i]; l = fmaf(t.y, __builtin_amdgcn_exp2f(t.x - mu), l); }
+    l = wave_sum(l);
+    if (threadIdx.x < D / 4) {
+        f4 sum = f4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < sp.n; ++i) {
+            const float e = __builtin_amdgcn_exp2f(sp.part_ml[r * sp.n + i].x - mu);
+            const f4 v = *reinterpret_cast<const f4*>(sp.part_o + (r * sp.n + i) * D + threadIdx.x * 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k] = fmaf(v[k], e, sum[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] = sum[k] / l;
+        *reinterpret_cast<f4*>(a.out + r * D + threadIdx.x * 4) = sum;
+    }
+    if (threadIdx.x == 0 && a.ml) a.ml[r] = float2{m, l};
+}
+// mass_out = mass_in + the softmax weights of one row, from the scores the attention left: 1024 positions a workgroup
+__global__ __launch_bounds__(256) void kv8_mass_scores_kernel(Kv8Attn a, Kv8Split sp) {
+    const int G = a.c.H / a.c.Hkv, hkv = blockIdx.y;
+    for (int t = blockIdx.x * 1024 + threadIdx.x, i = 0; i < 4 && t < a.mass_n; ++i, t += 256) {
+        float sum = 0.f;
+        for (int g = 0; g < G; ++g) {
+            const float2 ml = a.ml[hkv * G + g];
+            sum += __builtin_amdgcn_exp2f(sp.scores[(size_t)(hkv * G + g) * sp.scores_ld + t] - ml.x) / ml.y;
+        }
+        a.mass_out[(size_t)hkv * a.mass_ld + t] = a.mass_in[(size_t)hkv * a.mass_ld + t] + sum;
+    }
+}
+
 // ---------------------------------------------------------------- launchers
 #define KV8_BY_DIM(D, EXPR)                                   \
     switch (D) {                                              \
@@ -348,6 +612,16 @@ hipError_t launch_kv8_attn_rows(const Kv8Attn& a, hipStream_t st) {
 hipError_t launch_kv8_attn_mass(const Kv8Attn& a, hipStream_t st) {
     const unsigned blocks = (unsigned)((a.mass_n + kKv8Block - 1) / kKv8Block);
     KV8_BY_DIM(a.c.D, hipLaunchKernelGGL(kv8_attn_mass_kernel<kD>, dim3(blocks, a.c.Hkv), dim3(256), 0, st, a, kLog2e / sqrtf((float)kD)));
+    return hipGetLastError();
+}
+
+
+hipError_t launch_kv8_attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t st) {
+    const int cols = a.M * (a.c.H / a.c.Hkv);
+    const dim3 grid(sp.n, a.c.Hkv, (cols + 15) / 16);
+    KV8_BY_DIM(a.c.D, hipLaunchKernelGGL(kv8_attn_split_kernel<kD>, grid, dim3(256), 0, st, a, sp, kLog2e / sqrtf((float)kD)));
+    if (sp.n > 1) KV8_BY_DIM(a.c.D, hipLaunchKernelGGL(kv8_attn_join_kernel<kD>, dim3(a.M * a.c.H), dim3(64), 0, st, a, sp));
+    if (sp.scores) hipLaunchKernelGGL(kv8_mass_scores_kernel, dim3((a.mass_n + 1023) / 1024, a.c.Hkv), dim3(256), 0, st, a, sp);
     return hipGetLastError();
 }
 

@@ -7,6 +7,7 @@ namespace thk {
 
 static const int kKv8Block = 16;      // positions that share one K scale and one V scale per K/V head
 static const int kKv8Tile = 64;       // positions one step of the attention kernels takes: the cache is padded to whole tiles
+static const int kKv8SplitRows = 8192; // rows x splits whose parts the workspace holds
 static const int kKv8RowSlab = 2048;  // prompt rows one attention launch takes (sizes the per-row statistics)
 
 // Device memory of one cache.  n_blk = blocks per head, a multiple of 4 (whole tiles).
@@ -36,12 +37,22 @@ struct Kv8Attn {
     int mass_n;                       // entries per head that are written: all positions of the call, also those this slab's rows do not see yet
 };
 
+// Few rows over a long axis: the positions are cut into n parts of whole tiles, joined by a second launch when n > 1.
+struct Kv8Split {
+    int n;
+    float* part_o;                    // [M H][n][D]
+    float2* part_ml;                  // [M H][n]
+    float* scores;                    // [H][scores_ld] base-2 scores of a single row, for the weight count; or null
+    int64_t scores_ld;
+};
+
 hipError_t launch_kv8_append(const Kv8View& c, const float* k, const float* v, int64_t pos, int64_t n, hipStream_t st);
 hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_out, float* v_out, hipStream_t st);
 hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recent, const float* mass_in, int64_t ld_in, float* mass_out, int64_t ld_out, int32_t* kept,
                              hipStream_t st);
 hipError_t launch_kv8_move(const Kv8View& src, const Kv8View& dst, int n_keep, const int32_t* kept, hipStream_t st);
 hipError_t launch_kv8_attn_rows(const Kv8Attn& a, hipStream_t st);
+hipError_t launch_kv8_attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t st);
 hipError_t launch_kv8_attn_mass(const Kv8Attn& a, hipStream_t st);
 
 }  // namespace thk
