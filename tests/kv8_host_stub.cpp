@@ -36,7 +36,7 @@ hipError_t launch_kv8_select(int Hkv, int T, int keep, int sink, int recent, con
     note("select %d %d %d %d %d %lld %lld", Hkv, T, keep, sink, recent, (long long)li, (long long)lo); return launched();
 }
 hipError_t launch_kv8_move(const Kv8View&, const Kv8View&, int keep, const int32_t*, hipStream_t) { note("move %d", keep); return launched(); }
-hipError_t launch_kv8_attn_rows(const Kv8Attn& a, hipStream_t) { note("rows %d %d", a.n_past, a.M); return launched(); }
+hipError_t launch_kv8_attn_tile(const Kv8Attn& a, hipStream_t) { note("tile %d %d", a.n_past, a.M); return launched(); }
 hipError_t launch_kv8_attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t) { note("split %d %d %d", a.n_past, a.M, sp.n); return launched(); }
 hipError_t launch_kv8_attn_mass(const Kv8Attn& a, hipStream_t) { note("mass %d %d %d%s", a.n_past, a.M, a.mass_n, a.mass_in == a.mass_out ? " in place" : ""); return launched(); }
 }

@@ -139,17 +139,19 @@ static int kv8_attention(thk_kv8* kv, const char* what, const float* q, int64_t 
         a.n_past = (int)(n_past + i); a.M = (int)(M - i < kKv8RowSlab ? M - i : kKv8RowSlab);
         if (mass_out) { a.ml = kv->ml; a.mass_in = mass_in; a.mass_out = mass_out; a.mass_ld = kv->n_ctx; a.mass_n = (int)(n_past + M); }
         const int64_t groups = ((int64_t)a.M * (a.c.H / a.c.Hkv) + 15) / 16 * a.c.Hkv;      // workgroups without a split
-        if (groups <= 1024) {
+        bool scored = false;
+        const char* ev = getenv("KV8_COLS");
+        if ((int64_t)a.M * (a.c.H / a.c.Hkv) <= (ev ? atoi(ev) : 64)) {
             Kv8Split sp{};
             const int64_t tiles = (a.n_past + a.M + kKv8Tile - 1) / kKv8Tile, most = (tiles + 3) / 4;
             int64_t n = 512 / groups;
             if (n > most) n = most;
             if (n > kKv8SplitRows / ((int64_t)a.M * a.c.H)) n = kKv8SplitRows / ((int64_t)a.M * a.c.H);
             sp.n = n < 1 ? 1 : (int)n; sp.part_o = kv->part_o; sp.part_ml = kv->part_ml;
-            if (mass_out && a.M == 1) { sp.scores = kv->scores; sp.scores_ld = (int64_t)a.c.n_blk * kKv8Block; }
+            if (mass_out && a.M == 1) { scored = true; sp.scores = kv->scores; sp.scores_ld = (int64_t)a.c.n_blk * kKv8Block; }
             HIPCHK(ctx, launch_kv8_attn_split(a, sp, ctx->stream));
-        } else HIPCHK(ctx, launch_kv8_attn_rows(a, ctx->stream));
-        if (mass_out && a.M > 1) HIPCHK(ctx, launch_kv8_attn_mass(a, ctx->stream));
+        } else HIPCHK(ctx, launch_kv8_attn_tile(a, ctx->stream));
+        if (mass_out && !scored) HIPCHK(ctx, launch_kv8_attn_mass(a, ctx->stream));
         mass_in = mass_out;
     }
     return THK_OK;

@@ -237,80 +237,7 @@ __global__ __launch_bounds__(256) void kv8_move_kernel(Kv8View s, Kv8View d, int
     else move_body<D, true>(s, d, n_keep, kept, sm, src);
 }
 
-// ---------------------------------------------------------------- attention, one workgroup per (row, head)
-// Block by block: 16 threads share a position's score, then every thread adds its dimension's share with the running maximum and sum
-// of the softmax.  Scores carry log2(e), so that the weights are exp2.
-static const float kLog2e = 1.44269504088896340736f;
-template <int D>
-__device__ __forceinline__ float block_score(const Kv8View& c, const float* q, int hkv, int b, float scale) {     // of position 16 b + tid / 16, in all 16 threads of it
-    const size_t hb = (size_t)hkv * c.n_blk + b;
-    const int8_t* k = c.k + hb * (kKv8Block * D) + threadIdx.x * (D / 16);
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) s = fmaf((float)k[i], q[(threadIdx.x & 15) * (D / 16) + i], s);
-    return row16_sum(s) * (c.ks[hb] * scale);
-}
-template <int D>
-__global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Kv8Attn a, float scale) {
-    __shared__ float qs[D], ss[16], acc[256];
-    const Kv8View& c = a.c;
-    const int h = blockIdx.x, row = blockIdx.y, hkv = h / (c.H / c.Hkv), tid = threadIdx.x, T = a.n_past + row + 1;
-    const float* q = a.q + ((size_t)row * c.H + h) * D;
-    for (int d = tid; d < D; d += 256) qs[d] = q[d];
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    constexpr int NG = 256 / D, PT = 16 / NG;                               // thread: dimension tid % D, positions (tid / D) * PT + i of the block
-    for (int b = 0; b * kKv8Block < T; ++b) {
-        const float s = block_score<D>(c, qs, hkv, b, scale);
-        if ((tid & 15) == 0) ss[tid >> 4] = b * kKv8Block + (tid >> 4) < T ? s : -INFINITY;
-        __syncthreads();
-        float mb = m;
-#pragma unroll
-        for (int t = 0; t < 16; ++t) mb = fmaxf(mb, ss[t]);
-        const float mu = mb == -INFINITY ? 0.f : mb, al = exp2f(m - mu);
-        const size_t hb = (size_t)hkv * c.n_blk + b;
-        const int8_t* v = c.v + hb * (kKv8Block * D) + (tid % D) * 16 + (tid / D) * PT;
-        const float vs = c.vs[hb];
-        float ob = 0.f, lb = 0.f;
-#pragma unroll
-        for (int t = 0; t < 16; ++t) lb += exp2f(ss[t] - mu);
-#pragma unroll
-        for (int i = 0; i < PT; ++i) ob = fmaf(exp2f(ss[(tid / D) * PT + i] - mu), (float)v[i], ob);
-        o = fmaf(o, al, ob * vs); l = fmaf(l, al, lb); m = mb;
-        __syncthreads();
-    }
-    acc[tid] = o;
-    __syncthreads();
-    if (tid < D) {
-        float t = 0.f;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) t += acc[g * D + tid];
-        a.out[((size_t)row * c.H + h) * D + tid] = t / l;
-    }
-    if (tid == 0 && a.ml) a.ml[(size_t)row * c.H + h] = float2{m, l};
-}
-// mass_out = mass_in + the softmax weights of every row and head of the group; one workgroup per block and K/V head, rows and heads in order
-template <int D>
-__global__ __launch_bounds__(256) void kv8_attn_mass_kernel(Kv8Attn a, float scale) {
-    __shared__ float qs[D];
-    const Kv8View& c = a.c;
-    const int b = blockIdx.x, hkv = blockIdx.y, G = c.H / c.Hkv, tid = threadIdx.x, t = b * kKv8Block + (tid >> 4);
-    float sum = 0.f;
-    for (int row = 0; row < a.M; ++row) {
-        if (b * kKv8Block > a.n_past + row) continue;
-        for (int g = 0; g < G; ++g) {
-            const int h = hkv * G + g;
-            __syncthreads();
-            for (int d = tid; d < D; d += 256) qs[d] = a.q[((size_t)row * c.H + h) * D + d];
-            __syncthreads();
-            const float s = block_score<D>(c, qs, hkv, b, scale);
-            const float2 ml = a.ml[(size_t)row * c.H + h];
-            if (t <= a.n_past + row) sum += exp2f(s - ml.x) / ml.y;
-        }
-    }
-    if ((tid & 15) == 0 && t < a.mass_n) a.mass_out[(size_t)hkv * a.mass_ld + t] = a.mass_in[(size_t)hkv * a.mass_ld + t] + sum;
-}
-
+static const float kLog2e = 1.44269504088896340736f;      // scores carry log2(e): the weights are exp2
 
 // ---------------------------------------------------------------- attention of few rows: i8 matrix instructions, split over the positions
 // out_n = sum_t p_nt v_t with p = softmax(q_n . k_t), for up to 16 (row, head) columns n that read one K/V head.  Both products run on
@@ -575,6 +502,309 @@ __global__ __launch_bounds__(256) void kv8_mass_scores_kernel(Kv8Attn a, Kv8Spli
     }
 }
 
+// ---------------------------------------------------------------- attention of many rows: f16 matrix instructions, tiles shared through LDS
+// Many rows make the products the bound, and the digits' i32 sums would have to be joined for every tile; here the f32 operand is two f16
+// parts (hi + lo: 22 bits) on v_mfma_f32_16x16x32_f16 and the sums stay in f32 accumulators.  The codes become f16 exactly, once per workgroup
+// and tile, on their way into LDS.  A workgroup of 4 waves takes 64 NC columns (row, head of the group), each wave 16 NC of them.
+//   q       scaled by a power of two per column so that its largest entry is in [2^14, 2^15): both parts stay far from f16's ends
+//   weights p * v_scale in units of 2^(ref - 15), ref >= the exponent of the largest weight the column has met (relative to its running
+//           maximum): at most 2^15, and what the lo part cannot hold is below 2^-40 of that largest weight.  The accumulators are rescaled
+//           only where the running maximum or ref moves, which a wave skips when none of its columns did.
+typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
+struct HF8x2 { hf8 a, b; };
+// 16 codes -> 16 f16: byte + 128 behind 0x64 is 1024 + byte + 128 exactly, less 1152
+__device__ __forceinline__ HF8x2 codes_f16(i4 q) {
+    unsigned o[8];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const unsigned u = (unsigned)q[w] ^ 0x80808080u;
+        o[2 * w] = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+        o[2 * w + 1] = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(hf2, o[i]) - hf2{(_Float16)1152.f, (_Float16)1152.f});
+    HF8x2 r;
+    const uint4 lo = {o[0], o[1], o[2], o[3]}, hi = {o[4], o[5], o[6], o[7]};
+    r.a = __builtin_bit_cast(hf8, lo); r.b = __builtin_bit_cast(hf8, hi);
+    return r;
+}
+// hi and lo parts of eight f32; the empty asm keeps hi the rounding of the f32 value in both of its uses
+__device__ __forceinline__ void split_f16(const float (&x)[8], hf8& hi, hf8& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float v = x[i];
+        asm("" : "+v"(v));
+        hi[i] = (_Float16)v;
+        lo[i] = (_Float16)(v - (float)hi[i]);
+    }
+}
+// The B operand of q for one column: parts of dimensions (lane / 16) * D/4 + 8 st + j, st = 0 .. D/32 - 1.  Returns 1 / the power of two.
+template <int D>
+__device__ __forceinline__ float load_q_f16(const float* q, bool valid, hf8 (&hi)[D / 32], hf8 (&lo)[D / 32]) {
+    float x[D / 4];
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+        const f4 v = valid ? reinterpret_cast<const f4*>(q)[i] : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { x[4 * i + j] = v[j]; const unsigned a = abs_bits(v[j]); m = a > m ? a : m; }
+    }
+    m = chunks_max_bits(m);
+    const float amax = as_f(m);
+    const bool fine = amax >= 0x1p-100f && m < 0x7F800000u;
+    const int e = fine ? __builtin_amdgcn_frexp_expf(amax) : 15;
+    const float up = fine ? ldexpf(1.f, 15 - e) : 0.f;
+#pragma unroll
+    for (int st = 0; st < D / 32; ++st) {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = fine ? x[8 * st + j] * up : 0.f;
+        split_f16(y, hi[st], lo[st]);
+    }
+    return m >= 0x7F800000u ? as_f(0x7FC00000u) : ldexpf(1.f, e - 15);
+}
+// consecutive logical indices on one XCD (workgroups are dealt to the 8 XCDs in turn): neighbours share a head's codes in that XCD's L2
+__device__ __forceinline__ int xcd_order(int id, int n) {
+    const int q = n / 8, r = n % 8, x = id % 8;
+    return x * q + (x < r ? x : r) + id / 8;
+}
+
+template <int D, int NC>
+__global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int blocks, float scale) {
+    constexpr int ST = D / 32, NG = D / 16, KF = 4 * ST, VF = 2 * NG, PIECES = (D / 64 * 4 + NG) / 4;      // f16 fragments of a tile; 16-byte pieces a thread stages
+    extern __shared__ __align__(16) char smem[];
+    hf8* frag = reinterpret_cast<hf8*>(smem);                              // [2][KF + VF][64]: K fragments (group, step), V fragments (dimensions, half)
+    const Kv8View& c = a.c;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, ch = lane >> 4;
+    const int id = xcd_order(blockIdx.x, gridDim.x), hkv = id / blocks, blk = blocks - 1 - id % blocks;       // longest rows first
+    const int G = c.H / c.Hkv, cols = a.M * G, col0 = blk * 64 * NC, wcol0 = col0 + w * 16 * NC;
+    const int T = a.n_past + (min(col0 + 64 * NC, cols) - 1) / G + 1, tiles = (T + kKv8Tile - 1) / kKv8Tile;
+    const int wrow0 = wcol0 / G, wrow1 = (min(wcol0 + 16 * NC, cols) - 1) / G;                             // rows this wave holds (none: wcol0 >= cols)
+    const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + 16 * (n >> 2) + (n & 3)) * D + ch * (D / 4);
+    const int8_t* vb = c.v + (((size_t)hkv * c.n_blk + ch) * D + n) * 16;
+    const float *ksb = c.ks + (size_t)hkv * c.n_blk + ch, *vsb = c.vs + (size_t)hkv * c.n_blk + ch;
+
+    // piece p of a tile: K group p / (D/64), chunk p % (D/64), or V dimensions 16 (p - 4 D/64); wave w stages pieces w, w + 4, ...
+    i4 st[PIECES];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const int p = 4 * j + w;
+            const int8_t* src = p < 4 * (D / 64) ? kb + (size_t)t * (kKv8Tile * D) + 4 * (p / (D / 64)) * D + (p % (D / 64)) * 16 : vb + (size_t)t * (kKv8Tile * D) + (p - 4 * (D / 64)) * 256;
+            st[j] = *reinterpret_cast<const i4*>(src);
+        }
+    };
+    auto stage = [&](int buf) {
+        hf8* f = frag + (size_t)buf * (KF + VF) * 64 + lane;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const int p = 4 * j + w;
+            const HF8x2 h = codes_f16(st[j]);
+            f[(2 * p) * 64] = h.a;                                         // K: fragment group * ST + 2 chunk (+ 1); V: KF + 2 dims (+ 1): both 2 p
+            f[(2 * p + 1) * 64] = h.b;
+        }
+    };
+    fetch(0);
+    hf8 qh[NC][ST], ql[NC][ST];
+    float qf[NC], m[NC], l[NC];
+    int ref[NC], lim[NC];
+    f4 o[NC][NG];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+        const int col = wcol0 + 16 * k + n;
+        const bool valid = col < cols;
+        lim[k] = valid ? a.n_past + col / G : T - 1;
+        qf[k] = load_q_f16<D>(a.q + (valid ? (size_t)(col / G) * c.H + hkv * G + col % G : 0) * D + ch * (D / 4), valid, qh[k], ql[k]) * scale;
+        m[k] = -INFINITY; l[k] = 0.f; ref[k] = -1000;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) o[k][g] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    stage(0);
+    float ks = ksb[0], vs = vsb[0];
+    __syncthreads();
+    for (int t = 0; t < tiles; ++t) {
+        const bool more = t + 1 < tiles;
+        float ksn = 0.f, vsn = 0.f;
+        if (more) { fetch(t + 1); ksn = ksb[(size_t)(t + 1) * 4]; vsn = vsb[(size_t)(t + 1) * 4]; }
+        if (wcol0 < cols && t * kKv8Tile <= a.n_past + wrow1) {             // some row of this wave sees the tile
+            const hf8* kf_ = frag + (size_t)(t & 1) * (KF + VF) * 64 + lane;
+            const hf8* vf_ = kf_ + KF * 64;
+            f4 s[NC][4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+#pragma unroll
+                for (int k = 0; k < NC; ++k) s[k][g] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < ST; ++i) {
+                    const hf8 kk = kf_[(g * ST + i) * 64];
+#pragma unroll
+                    for (int k = 0; k < NC; ++k) {
+                        s[k][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[k][i], s[k][g], 0, 0, 0);
+                        s[k][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[k][i], s[k][g], 0, 0, 0);
+                    }
+                }
+            }
+            hf8 ph[NC][2], pl[NC][2];
+            const int pos = t * kKv8Tile + ch * 16;
+            const bool edge = t * kKv8Tile + kKv8Tile - 1 > a.n_past + wrow0;
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                const float kf = qf[k] * ks;
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[k][i >> 2][i & 3] = pos + i <= lim[k] ? s[k][i >> 2][i & 3] : -INFINITY;
+                }
+                float top = s[k][0][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top = fmaxf(top, s[k][i >> 2][i & 3]);
+                top = pos <= lim[k] ? top * kf : -INFINITY;                // kf >= 0, but 0 * -inf is NaN
+                const float mn = fmaxf(m[k], chunks_max(top)), mu = mn == -INFINITY ? 0.f : mn;
+                float p[16], ls = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p[i] = __builtin_amdgcn_exp2f(fmaf(s[k][i >> 2][i & 3], kf, -mu));
+                    if (edge) p[i] = pos + i <= lim[k] ? p[i] : 0.f;
+                    ls += p[i];
+                }
+                const float vsu = pos <= lim[k] ? vs : 0.f;
+                const unsigned wm = chunks_max_bits(as_u(__builtin_amdgcn_exp2f(top - mu) * vsu));
+                const int e = wm >= 0x7F800000u ? 1000 : wm == 0 ? -1000 : __builtin_amdgcn_frexp_expf(as_f(wm));
+                if (__any(mn != m[k] || e > ref[k])) {                      // NaN maxima compare unequal: rescaled each time, harmless
+                    const float al = __builtin_amdgcn_exp2f(m[k] - mu);
+                    const int shrunk = ref[k] + (al > 0.f ? __builtin_amdgcn_frexp_expf(al) - 1 : -1000), rn = max(max(shrunk, e), -1000);
+                    const float f = ldexpf(al, max(min(ref[k] - rn, 2000), -2000));
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[k][g][i] *= f;
+                    l[k] *= al; m[k] = mn; ref[k] = rn;
+                }
+                l[k] += ls;
+                const float fac = ldexpf(vsu, 15 - ref[k]) + (as_f(wm) - as_f(wm));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = p[8 * h + i] * fac;
+                    split_f16(x, ph[k][h], pl[k][h]);
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const hf8 vv = vf_[(g * 2 + h) * 64];
+#pragma unroll
+                    for (int k = 0; k < NC; ++k) {
+                        o[k][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[k][h], o[k][g], 0, 0, 0);
+                        o[k][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[k][h], o[k][g], 0, 0, 0);
+                    }
+                }
+        }
+        if (more) { stage((t + 1) & 1); ks = ksn; vs = vsn; }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+        const int col = wcol0 + 16 * k + n;
+        if (col >= cols) continue;
+        const size_t r = (size_t)(col / G) * c.H + hkv * G + col % G;
+        const float lt = chunks_sum(l[k]), f = ldexpf(1.f, max(ref[k], -200) - 15) / lt;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) *reinterpret_cast<f4*>(a.out + r * D + 16 * g + 4 * ch) = o[k][g] * f;
+        if (a.ml && ch == 0) a.ml[r] = float2{m[k], lt};
+    }
+}
+
+// ---------------------------------------------------------------- weight count of many rows
+// mass_out = mass_in + sum over the columns of exp2(s - m) / l: a wave keeps the K fragments of 16 TG positions in registers and walks the
+// columns, whose q parts the workgroup stages 64 at a time; columns sum in a fixed order.
+template <int D, int TG>
+__global__ __launch_bounds__(256, 2) void kv8_mass_tile_kernel(Kv8Attn a, float scale) {
+    constexpr int ST = D / 32;
+    extern __shared__ __align__(16) char smem[];
+    hf8* qs = reinterpret_cast<hf8*>(smem);                                // [4 column groups][2 parts][ST][64]
+    float2* stat = reinterpret_cast<float2*>(qs + 4 * 2 * ST * 64);        // [64]: q factor / maximum
+    float* rl = reinterpret_cast<float*>(stat + 64);                       // [64]: 1 / sum
+    const Kv8View& c = a.c;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, ch = lane >> 4, hkv = blockIdx.y, G = c.H / c.Hkv, cols = a.M * G;
+    // wave's positions: TG == 4: tile 4 blockIdx.x + w, lane chunk ch and score 4 g + i is position 16 ch + 4 g + i of it;
+    // TG == 1: group w of tile blockIdx.x: position 16 ch + 4 w + i
+    const int tile = TG == 4 ? blockIdx.x * 4 + w : blockIdx.x, g0 = TG == 4 ? 0 : w, first = (TG == 4 ? blockIdx.x * 4 : blockIdx.x) * kKv8Tile;
+    const bool live = tile * kKv8Tile < a.n_past + a.M;
+    const int pos = tile * kKv8Tile + ch * 16 + 4 * g0;
+    hf8 kk[TG][ST];
+    float ks = 0.f;
+    if (live) {
+        const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + (size_t)tile * kKv8Tile + 16 * (n >> 2) + (n & 3)) * D + ch * (D / 4);
+        ks = c.ks[(size_t)hkv * c.n_blk + (size_t)tile * 4 + ch];
+#pragma unroll
+        for (int g = 0; g < TG; ++g)
+#pragma unroll
+            for (int kc = 0; kc < D / 64; ++kc) {
+                const HF8x2 h = codes_f16(*reinterpret_cast<const i4*>(kb + 4 * (g0 + g) * D + kc * 16));
+                kk[g][2 * kc] = h.a; kk[g][2 * kc + 1] = h.b;
+            }
+    }
+    float sum[TG * 4];
+#pragma unroll
+    for (int i = 0; i < TG * 4; ++i) sum[i] = 0.f;
+    const int row0 = max(first - a.n_past, 0);                             // the first row that sees a position of this workgroup
+    for (int c0 = row0 * G / 64 * 64; c0 < cols; c0 += 64) {
+        const int col = c0 + w * 16 + n;
+        const bool valid = col < cols;
+        const size_t r = valid ? (size_t)(col / G) * c.H + hkv * G + col % G : 0;
+        hf8 hi[ST], lo[ST];
+        const float f = load_q_f16<D>(a.q + r * D + ch * (D / 4), valid, hi, lo) * scale;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < ST; ++i) { qs[(w * 2 * ST + i) * 64 + lane] = hi[i]; qs[(w * 2 * ST + ST + i) * 64 + lane] = lo[i]; }
+        if (ch == 0) { const float2 t = valid ? a.ml[r] : float2{0.f, 1.f}; stat[w * 16 + n] = float2{f, t.x}; rl[w * 16 + n] = valid ? 1.f / t.y : 0.f; }
+        __syncthreads();
+        if (!live) continue;
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+            if (c0 + q * 16 >= cols) break;
+            const float2 sf = stat[q * 16 + n];
+            const float inv = rl[q * 16 + n], kf = sf.x * ks;
+            const int lim = a.n_past + min((c0 + q * 16 + n) / G, a.M - 1);
+            const hf8* qq = qs + (q * 2 * ST) * 64 + lane;
+            f4 s[TG];
+#pragma unroll
+            for (int g = 0; g < TG; ++g) s[g] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < ST; ++i) {
+                const hf8 qh = qq[i * 64], ql = qq[(ST + i) * 64];
+#pragma unroll
+                for (int g = 0; g < TG; ++g) {
+                    s[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[g][i], qh, s[g], 0, 0, 0);
+                    s[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[g][i], ql, s[g], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < TG * 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], kf, -sf.y)) * inv;
+                sum[i] += pos + i <= lim && c0 + q * 16 + n < cols ? p : 0.f;
+            }
+        }
+    }
+    if (!live) return;
+#pragma unroll
+    for (int i = 0; i < TG * 4; ++i) {
+        const float t = row16_sum(sum[i]);
+        if (n == i) {
+            const size_t at = (size_t)hkv * a.mass_ld + pos + i;
+            if (pos + i < a.n_past + a.M) a.mass_out[at] = a.mass_in[at] + t;
+        }
+    }
+}
+// entries behind the slab's positions: carried over
+__global__ __launch_bounds__(256) void kv8_mass_rest_kernel(Kv8Attn a) {
+    const int t = a.n_past + a.M + blockIdx.x * 256 + threadIdx.x;
+    if (t < a.mass_n) a.mass_out[(size_t)blockIdx.y * a.mass_ld + t] = a.mass_in[(size_t)blockIdx.y * a.mass_ld + t];
+}
+
 // ---------------------------------------------------------------- launchers
 #define KV8_BY_DIM(D, EXPR)                                   \
     switch (D) {                                              \
@@ -605,17 +835,42 @@ hipError_t launch_kv8_move(const Kv8View& src, const Kv8View& dst, int n_keep, c
     KV8_BY_DIM(src.D, hipLaunchKernelGGL(kv8_move_kernel<kD>, grid, dim3(256), 0, st, src, dst, n_keep, kept));
     return hipGetLastError();
 }
-hipError_t launch_kv8_attn_rows(const Kv8Attn& a, hipStream_t st) {
-    KV8_BY_DIM(a.c.D, hipLaunchKernelGGL(kv8_attn_rows_kernel<kD>, dim3(a.c.H, a.M), dim3(256), 0, st, a, kLog2e / sqrtf((float)kD)));
+template <typename F> static hipError_t lds_opt_in(F kernel, size_t bytes) {
+    return bytes > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : hipSuccess;
+}
+template <int D> static hipError_t attn_tile(const Kv8Attn& a, hipStream_t st) {
+    constexpr int NC = D == 256 ? 1 : 2;
+    constexpr size_t lds = (size_t)2 * (4 * (D / 32) + 2 * (D / 16)) * 64 * 16;
+    const int cols = a.M * (a.c.H / a.c.Hkv), blocks = (cols + 64 * NC - 1) / (64 * NC);
+    const hipError_t e = lds_opt_in(kv8_attn_tile_kernel<D, NC>, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<D, NC>), dim3(blocks * a.c.Hkv), dim3(256), lds, st, a, blocks, kLog2e / sqrtf((float)D));
+    return hipGetLastError();
+}
+hipError_t launch_kv8_attn_tile(const Kv8Attn& a, hipStream_t st) {
+    KV8_BY_DIM(a.c.D, return attn_tile<kD>(a, st));
+    return hipErrorInvalidValue;
+}
+template <int D> static hipError_t mass_tile(const Kv8Attn& a, hipStream_t st) {
+    constexpr size_t lds = (size_t)4 * 2 * (D / 32) * 64 * 16 + 64 * 12;
+    const int tiles = (a.n_past + a.M + kKv8Tile - 1) / kKv8Tile;
+    if (tiles * a.c.Hkv >= 2048) {
+        const hipError_t e = lds_opt_in(kv8_mass_tile_kernel<D, 4>, lds);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((kv8_mass_tile_kernel<D, 4>), dim3((tiles + 3) / 4, a.c.Hkv), dim3(256), lds, st, a, kLog2e / sqrtf((float)D));
+    } else {
+        const hipError_t e = lds_opt_in(kv8_mass_tile_kernel<D, 1>, lds);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((kv8_mass_tile_kernel<D, 1>), dim3(tiles, a.c.Hkv), dim3(256), lds, st, a, kLog2e / sqrtf((float)D));
+    }
+    const int rest = a.mass_n - (a.n_past + a.M);
+    if (rest > 0 && a.mass_in != a.mass_out) hipLaunchKernelGGL(kv8_mass_rest_kernel, dim3((rest + 255) / 256, a.c.Hkv), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 hipError_t launch_kv8_attn_mass(const Kv8Attn& a, hipStream_t st) {
-    const unsigned blocks = (unsigned)((a.mass_n + kKv8Block - 1) / kKv8Block);
-    KV8_BY_DIM(a.c.D, hipLaunchKernelGGL(kv8_attn_mass_kernel<kD>, dim3(blocks, a.c.Hkv), dim3(256), 0, st, a, kLog2e / sqrtf((float)kD)));
-    return hipGetLastError();
+    KV8_BY_DIM(a.c.D, return mass_tile<kD>(a, st));
+    return hipErrorInvalidValue;
 }
-
-
 hipError_t launch_kv8_attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t st) {
     const int cols = a.M * (a.c.H / a.c.Hkv);
     const dim3 grid(sp.n, a.c.Hkv, (cols + 15) / 16);

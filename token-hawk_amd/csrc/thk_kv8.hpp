@@ -51,7 +51,7 @@ hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_ou
 hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recent, const float* mass_in, int64_t ld_in, float* mass_out, int64_t ld_out, int32_t* kept,
                              hipStream_t st);
 hipError_t launch_kv8_move(const Kv8View& src, const Kv8View& dst, int n_keep, const int32_t* kept, hipStream_t st);
-hipError_t launch_kv8_attn_rows(const Kv8Attn& a, hipStream_t st);
+hipError_t launch_kv8_attn_tile(const Kv8Attn& a, hipStream_t st);
 hipError_t launch_kv8_attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t st);
 hipError_t launch_kv8_attn_mass(const Kv8Attn& a, hipStream_t st);
 
