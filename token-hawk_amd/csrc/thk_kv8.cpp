@@ -12,6 +12,7 @@ struct thk_kv8 {
     float2* ml = nullptr;       // per-row softmax statistics of an attention call that counts weights
     float* part_o = nullptr;    // parts of rows that are split over the positions
     float2* part_ml = nullptr;
+    unsigned* counters = nullptr;
     float* scores = nullptr;    // [H][padded n_ctx]: a single row's scores, for the weight count
 };
 
@@ -57,7 +58,7 @@ extern "C" int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_
     const size_t codes = (size_t)H_kv * v.n_blk * kKv8Block * D, scales = up256((size_t)H_kv * v.n_blk * 4), tail = (size_t)2 * H_kv * kKv8Block * D * 4;
     const size_t at = up256((size_t)2 * H_kv * sizeof(int2)), ml = (size_t)kKv8RowSlab * H * sizeof(float2);
     const size_t part = (size_t)kKv8SplitRows * (D * 4 + sizeof(float2)), scores_bytes = (size_t)H * v.n_blk * kKv8Block * 4;
-    kv->mem_bytes = 2 * codes + 2 * scales + tail + at + ml + part + scores_bytes;
+    kv->mem_bytes = 2 * codes + 2 * scales + tail + at + ml + part + kKv8Counters * 4 + scores_bytes;
     hipError_t e = hipMalloc(&kv->mem, kv->mem_bytes);
     if (e != hipSuccess) {
         (void)hipGetLastError();
@@ -75,6 +76,7 @@ extern "C" int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_
     kv->ml = (float2*)p; p += ml;
     kv->part_o = (float*)p; p += (size_t)kKv8SplitRows * D * 4;
     kv->part_ml = (float2*)p; p += (size_t)kKv8SplitRows * sizeof(float2);
+    kv->counters = (unsigned*)p; p += kKv8Counters * 4;
     kv->scores = (float*)p;
     e = hipMemsetAsync(kv->mem, 0, kv->mem_bytes, ctx->stream);
     if (e == hipSuccess) e = hipMemsetAsync(v.tail_at, 0xFF, (size_t)2 * H_kv * sizeof(int2), ctx->stream);     // no block is open
@@ -138,17 +140,22 @@ static int kv8_attention(thk_kv8* kv, const char* what, const float* q, int64_t 
         a.c = kv->view; a.q = q + i * row; a.out = out + i * row;
         a.n_past = (int)(n_past + i); a.M = (int)(M - i < kKv8RowSlab ? M - i : kKv8RowSlab);
         if (mass_out) { a.ml = kv->ml; a.mass_in = mass_in; a.mass_out = mass_out; a.mass_ld = kv->n_ctx; a.mass_n = (int)(n_past + M); }
-        const int64_t groups = ((int64_t)a.M * (a.c.H / a.c.Hkv) + 15) / 16 * a.c.Hkv;      // workgroups without a split
         bool scored = false;
-        const char* ev = getenv("KV8_COLS");
-        if ((int64_t)a.M * (a.c.H / a.c.Hkv) <= (ev ? atoi(ev) : 64)) {
+        const int64_t G = a.c.H / a.c.Hkv, cols = a.M * G, cg = (cols + 15) / 16, groups = cg * a.c.Hkv;      // workgroups without a split
+        auto env = [](const char* n, int64_t d) { const char* e = getenv(n); return e ? (int64_t)atoll(e) : d; };
+        if (cols <= env("KV8_COLS", 64)) {
             Kv8Split sp{};
-            const int64_t tiles = (a.n_past + a.M + kKv8Tile - 1) / kKv8Tile, most = (tiles + 3) / 4;
-            int64_t n = 512 / groups;
+            sp.waves = a.c.D == 256 ? 4 : (int)env("KV8_W", 8);
+            const int64_t T = a.n_past + a.M, tiles = (T + kKv8Tile - 1) / kKv8Tile, most = (tiles + sp.waves - 1) / sp.waves;
+            int64_t n = env("KV8_WG", sp.waves == 8 ? 256 : 512) / groups;
             if (n > most) n = most;
+            if (n > 64) n = 64;
             if (n > kKv8SplitRows / ((int64_t)a.M * a.c.H)) n = kKv8SplitRows / ((int64_t)a.M * a.c.H);
             sp.n = n < 1 ? 1 : (int)n; sp.part_o = kv->part_o; sp.part_ml = kv->part_ml;
-            if (mass_out && a.M == 1) { scored = true; sp.scores = kv->scores; sp.scores_ld = (int64_t)a.c.n_blk * kKv8Block; }
+            sp.stream = cg == 1 && 2 * T * a.c.Hkv * a.c.D >= env("KV8_NTB", 64 << 20);
+            if (mass_out && a.M == 1 && G <= 16) { scored = true; sp.scores = kv->scores; sp.scores_ld = (int64_t)a.c.n_blk * kKv8Block; }
+            const bool join = sp.n * std::min<int64_t>(cols, 16) <= env("KV8_JOIN", 64) && (!scored || T * G <= env("KV8_JOINT", 8192));
+            if (groups <= kKv8Counters && join && (sp.n > 1 || scored)) sp.counters = kv->counters;
             HIPCHK(ctx, launch_kv8_attn_split(a, sp, ctx->stream));
         } else HIPCHK(ctx, launch_kv8_attn_tile(a, ctx->stream));
         if (mass_out && !scored) HIPCHK(ctx, launch_kv8_attn_mass(a, ctx->stream));

@@ -2,6 +2,7 @@
 // Layout: thk_kv8.hpp.  All sums, softmax statistics and scales are f32; the codes are the only 8-bit values.
 #include "thk_device.hpp"
 #include "thk_kv8.hpp"
+#include <type_traits>
 
 namespace thk {
 
@@ -250,6 +251,11 @@ static const float kLog2e = 1.44269504088896340736f;      // scores carry log2(e
 // lane chunk c ends up with the scores of the 16 positions of block c: then one K scale and one V scale per lane serve a whole tile, and
 // the second product's B operand is what the lane already holds - no exchange between lanes.
 typedef int i4 __attribute__((ext_vector_type(4)));
+#ifdef KV8_NT
+__device__ __forceinline__ i4 LD(const void* p) { return __builtin_nontemporal_load(reinterpret_cast<const i4*>(p)); }
+#else
+__device__ __forceinline__ i4 LD(const void* p) { return *reinterpret_cast<const i4*>(p); }
+#endif
 struct U2 { unsigned a, b; };
 // Between them, a and b hold a value and that of the lane 16 (32) away, in every lane.  The swap works on two registers: the empty asm keeps
 // the compiler from giving it the same one twice, which would leave the value where it is.
@@ -283,60 +289,74 @@ __device__ __forceinline__ float chunks_sum(float v) {
     r = pair32(as_u(as_f(r.a) + as_f(r.b)));
     return as_f(r.a) + as_f(r.b);
 }
-// Four numbers given as x + 0x808080 (x = d2 2^16 + d1 2^8 + d0, the low three bytes are the digits plus 128): their digits, four to a word.
+// Four numbers whose low two bytes are digits plus 128 (x + 0x8080 for x >= 0, x + 0x808080 with SIGNED: then the third byte too): their
+// digits, four to a word.
+template <bool SIGNED>
 __device__ __forceinline__ void pack_digits(unsigned e0, unsigned e1, unsigned e2, unsigned e3, int& d2, int& d1, int& d0) {
     const unsigned a = __builtin_amdgcn_perm(e1, e0, 0x05040100u), b = __builtin_amdgcn_perm(e3, e2, 0x05040100u);     // bytes: e0.0 e0.1 e1.0 e1.1
     const unsigned u = __builtin_amdgcn_perm(e1, e0, 0x0C0C0602u), w = __builtin_amdgcn_perm(e3, e2, 0x06020C0Cu);
     d0 = (int)(__builtin_amdgcn_perm(b, a, 0x06040200u) ^ 0x80808080u);
     d1 = (int)(__builtin_amdgcn_perm(b, a, 0x07050301u) ^ 0x80808080u);
-    d2 = (int)((u | w) ^ 0x80808080u);
+    d2 = (int)(SIGNED ? (u | w) ^ 0x80808080u : u | w);
 }
 __device__ __forceinline__ float join_digits(int i2, int i1, int i0) { return fmaf((float)i2, 65536.f, (float)(i1 * 256 + i0)); }   // |i1| <= 256 * 2^14: no overflow
 
-// The B operand of q: digits of columns n = 16 cg + lane % 16, dimensions (lane / 16) * D/4 + 16 kc + j.  Returns the step of the fixed point.
+// The B operand of q: digits of columns n = 16 cg + lane % 16, dimensions 64 kc + 16 (lane / 16) + j.  Returns the step of the fixed point.
 template <int D>
-__device__ __forceinline__ float load_q_digits(const float* q, bool valid, i4 (&qd)[3][D / 64]) {
-    float x[D / 4];
+__device__ __forceinline__ void load_q(const float* q, bool valid, f4 (&x)[D / 16]) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) x[i] = valid ? reinterpret_cast<const f4*>(q)[(i / 4) * 16 + i % 4] : f4{0.f, 0.f, 0.f, 0.f};
+}
+template <int D>
+__device__ __forceinline__ float q_digits(const f4 (&x)[D / 16], i4 (&qd)[3][D / 64]) {
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-        const f4 v = valid ? reinterpret_cast<const f4*>(q)[i] : f4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { x[4 * i + j] = v[j]; const unsigned a = abs_bits(v[j]); m = a > m ? a : m; }
-    }
+        for (int j = 0; j < 4; ++j) { const unsigned a = abs_bits(x[i][j]); m = a > m ? a : m; }
     m = chunks_max_bits(m);
-    const float amax = __builtin_bit_cast(float, m);
+    const float amax = as_f(m);
     const bool some = amax >= 0x1p-100f;                                   // also false for NaN
     const float inv = some && m < 0x7F800000u ? 8355000.f / amax : 0.f;    // below 127 (2^16 + 2^8 + 1), the largest sum of three balanced digits, by more than the roundings
 #pragma unroll
-    for (int kc = 0; kc < D / 64; ++kc)
+    for (int i = 0; i < D / 16; ++i) {
+        unsigned e[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            unsigned e[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = (unsigned)((int)rintf(x[16 * kc + 4 * w + j] * inv) + 0x808080);
-            int d2, d1, d0;
-            pack_digits(e[0], e[1], e[2], e[3], d2, d1, d0);
-            qd[2][kc][w] = d2; qd[1][kc][w] = d1; qd[0][kc][w] = d0;
-        }
-    if (m >= 0x7F800000u) return __builtin_bit_cast(float, 0x7FC00000u);    // a query that is not finite: every score is NaN
+        for (int j = 0; j < 4; ++j) e[j] = (unsigned)((int)rintf(x[i][j] * inv) + 0x808080);
+        int d2, d1, d0;
+        pack_digits<true>(e[0], e[1], e[2], e[3], d2, d1, d0);
+        qd[2][i / 4][i % 4] = d2; qd[1][i / 4][i % 4] = d1; qd[0][i / 4][i % 4] = d0;
+    }
+    if (m >= 0x7F800000u) return as_f(0x7FC00000u);                        // a query that is not finite: every score is NaN
     return some ? amax / 8355000.f : 0.f;
 }
+// What one workgroup leaves for another inside a launch is written and read past the XCDs' own L2s (agent scope).
+__device__ __forceinline__ void put2(float* p, float x, float y) { st_agent_u64(reinterpret_cast<unsigned long long*>(p), (unsigned long long)as_u(y) << 32 | as_u(x)); }
+__device__ __forceinline__ float2 get2(const float* p) { const unsigned long long v = ld_agent_u64(reinterpret_cast<const unsigned long long*>(p)); return {as_f((unsigned)v), as_f((unsigned)(v >> 32))}; }
 
-template <int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_split_kernel(Kv8Attn a, Kv8Split sp, float scale) {
+template <bool NT> __device__ __forceinline__ i4 load16(const void* p) {
+    if (NT) return __builtin_nontemporal_load(reinterpret_cast<const i4*>(p));
+    return *reinterpret_cast<const i4*>(p);
+}
+// W waves, a tile each in turn.  NT: codes that will not be read again soon (many more than the caches hold) go past them.
+template <int D, int W, bool NT>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_attn_split_kernel(Kv8Attn a, Kv8Split sp, float scale) {
     constexpr int KC = D / 64, NG = D / 16;
-    __shared__ float so[4][16][D + 4], sml[4][16][2];
+    __shared__ float so[W][16][D + 4], sml[W][16][2];
+    __shared__ int last;
     const Kv8View& c = a.c;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, ch = lane >> 4;
     const int split = blockIdx.x, hkv = blockIdx.y, col = blockIdx.z * 16 + n, G = c.H / c.Hkv, cols = a.M * G;
-    const int row = col / G, last_col = min((int)blockIdx.z * 16 + 15, cols - 1);
-    const bool valid = col < cols;
-    const int T = a.n_past + last_col / G + 1, first_lim = a.n_past + (int)blockIdx.z * 16 / G, lim = valid ? a.n_past + row : T - 1;   // positions <= lim are seen
+    const bool valid = col < cols, one = a.M == 1;                   // one row: no division (a launch of a single token is short enough to feel them)
+    const int row = one ? 0 : col / G, last_row = one ? 0 : min((int)blockIdx.z * 16 + 15, cols - 1) / G;
+    const int T = a.n_past + last_row + 1, first_lim = one ? a.n_past : a.n_past + (int)blockIdx.z * 16 / G, lim = valid ? a.n_past + row : T - 1;   // positions <= lim are seen
     const int tiles = (T + kKv8Tile - 1) / kKv8Tile, per = (tiles + sp.n - 1) / sp.n, t1 = min((split + 1) * per, tiles);
-    const size_t orow = valid ? (size_t)row * c.H + hkv * G + col % G : 0;
+    const size_t orow = valid ? (size_t)row * c.H + hkv * G + (col - row * G) : 0;
+    auto out_row = [&](int cc) { const int i = one ? 0 : cc / G; return (size_t)i * c.H + hkv * G + (cc - i * G); };
 
-    const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + 16 * (n >> 2) + (n & 3)) * D + ch * (D / 4);
+    f4 qx[D / 16];
+    load_q<D>(a.q + orow * D + ch * 16, valid, qx);
+    const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + 16 * (n >> 2) + (n & 3)) * D + ch * 16;
     const int8_t* vb = c.v + (((size_t)hkv * c.n_blk + ch) * D + n) * 16;
     const float *ksb = c.ks + (size_t)hkv * c.n_blk + ch, *vsb = c.vs + (size_t)hkv * c.n_blk + ch;
     i4 kr[4][KC], vr[NG];
@@ -346,24 +366,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_split_kernel(K
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
-            for (int kc = 0; kc < KC; ++kc) kr[g][kc] = *reinterpret_cast<const i4*>(p + (4 * g) * D + kc * 16);
+            for (int kc = 0; kc < KC; ++kc) kr[g][kc] = load16<NT>(p + (4 * g) * D + kc * 64);
         ks = ksb[(size_t)t * 4];
     };
     auto load_v = [&](int t) {
         const int8_t* p = vb + (size_t)t * (kKv8Tile * D);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) vr[g] = *reinterpret_cast<const i4*>(p + g * 256);
+        for (int g = 0; g < NG; ++g) vr[g] = load16<NT>(p + g * 256);
         vs = vsb[(size_t)t * 4];
     };
     int t = split * per + w;
     if (t < t1) { load_k(t); load_v(t); }
     i4 qd[3][KC];
-    const float qf = load_q_digits<D>(a.q + orow * D + ch * (D / 4), valid, qd) * scale;
+    const float qf = q_digits<D>(qx, qd) * scale;
     float m = -INFINITY, l = 0.f;
     f4 o[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) o[g] = f4{0.f, 0.f, 0.f, 0.f};
-    for (; t < t1; t += 4) {
+    // One tile; `more` is a constant in each of its two uses: with a branch around the loads the compiler would wait for all of them wherever it
+    // waits for any.
+    auto step = [&](auto more) {
         float s[16];
         const float kf = qf * ks;
 #pragma unroll
@@ -379,31 +401,41 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_split_kernel(K
             for (int i = 0; i < 4; ++i) s[4 * g + i] = join_digits(acc[2][i], acc[1][i], acc[0][i]) * kf;
             if (g & 1) __builtin_amdgcn_sched_barrier(0);            // two groups in flight: more only cost registers
         }
-        const int tn = t + 4;
-        if (tn < t1) load_k(tn);
+        if (decltype(more)::value) load_k(t + W);
         const int pos = t * kKv8Tile + ch * 16;
         if (t * kKv8Tile + kKv8Tile - 1 > first_lim) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = pos + i <= lim ? s[i] : -INFINITY;
         }
         if (sp.scores && valid) {
-            f4* ps = reinterpret_cast<f4*>(sp.scores + orow * sp.scores_ld + pos);
+            float* ps = sp.scores + orow * sp.scores_ld + pos;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) ps[g] = f4{s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+            for (int i = 0; i < 16; i += 4) {
+                if (sp.counters) { put2(ps + i, s[i], s[i + 1]); put2(ps + i + 2, s[i + 2], s[i + 3]); }     // read in this launch
+                else *reinterpret_cast<f4*>(ps + i) = f4{s[i], s[i + 1], s[i + 2], s[i + 3]};
+            }
         }
         float sm = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) sm = fmaxf(sm, s[i]);
-        const float mn = fmaxf(m, chunks_max(sm)), mu = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - mu);
+        const float mn = fmaxf(m, chunks_max(sm)), mu = mn == -INFINITY ? 0.f : mn;
+        if (__any(mn != m)) {                                        // a new maximum in some column: rare after the first tiles
+            const float al = __builtin_amdgcn_exp2f(m - mu);
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[g][i] *= al;
+            l *= al;
+            m = mn;
+        }
         float ls = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(s[i] - mu); ls += s[i]; }
-        l = fmaf(l, al, ls);
-        m = mn;
+        l += ls;
         // weights p * vs in steps of 2^(e - 22), e the exponent of the tile's largest: whole numbers below 2^22.  Blocks no row of this
         // column sees (p = 0 throughout) must not bring in their scale, which may be NaN.
         const float vsu = pos <= lim ? vs : 0.f;
-        const float wm = __builtin_bit_cast(float, chunks_max_bits(__builtin_bit_cast(unsigned, __builtin_amdgcn_exp2f(sm - mu) * vsu)));
+        const float wm = as_f(chunks_max_bits(as_u(__builtin_amdgcn_exp2f(sm - mu) * vsu)));
         const int e = __builtin_amdgcn_frexp_expf(wm);
         const float fac = ldexpf(vsu, 22 - e), f = ldexpf(1.f, e - 22) + (wm - wm);                  // wm - wm: 0, or NaN if wm is not finite
         i4 pd[3];
@@ -411,9 +443,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_split_kernel(K
         for (int g = 0; g < 4; ++g) {
             unsigned x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __builtin_bit_cast(unsigned, fmaf(s[4 * g + i], fac, 8388608.f)) + 0x00808080u;
+            for (int i = 0; i < 4; ++i) x[i] = as_u(fmaf(s[4 * g + i], fac, 8421504.f));             // 2^23 + 0x8080: the mantissa is x + 0x8080
             int d2, d1, d0;
-            pack_digits(x[0], x[1], x[2], x[3], d2, d1, d0);
+            pack_digits<false>(x[0], x[1], x[2], x[3], d2, d1, d0);
             pd[2][g] = d2; pd[1][g] = d1; pd[0][g] = d0;
         }
 #pragma unroll
@@ -423,13 +455,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_split_kernel(K
             const i4 a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[g], pd[1], z, 0, 0, 0);
             const i4 a0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[g], pd[0], z, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[g][i] = fmaf(o[g][i], al, f * join_digits(a2[i], a1[i], a0[i]));
+            for (int i = 0; i < 4; ++i) o[g][i] = fmaf(f, join_digits(a2[i], a1[i], a0[i]), o[g][i]);
             if (g & 1) __builtin_amdgcn_sched_barrier(0);
         }
-        if (tn < t1) load_v(tn);
-    }
+        if (decltype(more)::value) load_v(t + W);
+    };
+    for (; t + W < t1; t += W) step(std::true_type{});
+    if (t < t1) step(std::false_type{});
     l = chunks_sum(l);
-    // join the four waves: columns n, dimensions 16 g + 4 ch + i
+    // join the waves: columns n, dimensions 16 g + 4 ch + i
     if (valid) {
 #pragma unroll
         for (int g = 0; g < NG; ++g) *reinterpret_cast<f4*>(&so[w][n][16 * g + 4 * ch]) = o[g];
@@ -437,14 +471,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_split_kernel(K
     }
     __syncthreads();
     const int nv = min(cols - (int)blockIdx.z * 16, 16);
-    for (int j = threadIdx.x; j < nv * (D / 4); j += 256) {
+    for (int j = threadIdx.x; j < nv * (D / 4); j += 64 * W) {
         const int cn = j / (D / 4), d = (j % (D / 4)) * 4, cc = blockIdx.z * 16 + cn;
-        const size_t r = (size_t)(cc / G) * c.H + hkv * G + cc % G;
-        const float mm = fmaxf(fmaxf(sml[0][cn][0], sml[1][cn][0]), fmaxf(sml[2][cn][0], sml[3][cn][0])), mu = mm == -INFINITY ? 0.f : mm;
+        const size_t r = out_row(cc);
+        float mm = sml[0][cn][0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) mm = fmaxf(mm, sml[i][cn][0]);
+        const float mu = mm == -INFINITY ? 0.f : mm;
         f4 sum = f4{0.f, 0.f, 0.f, 0.f};
         float ll = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < W; ++i) {
             const float e = __builtin_amdgcn_exp2f(sml[i][cn][0] - mu);
             const f4 v = *reinterpret_cast<const f4*>(&so[i][cn][d]);
 #pragma unroll
@@ -455,37 +492,92 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_split_kernel(K
 #pragma unroll
             for (int k = 0; k < 4; ++k) sum[k] = sum[k] / ll;
             *reinterpret_cast<f4*>(a.out + r * D + d) = sum;
-        } else {
+        } else if (!sp.counters) {
             *reinterpret_cast<f4*>(sp.part_o + (r * sp.n + split) * D + d) = sum;
+        } else {
+            float* po = sp.part_o + (r * sp.n + split) * D + d;
+            put2(po, sum[0], sum[1]); put2(po + 2, sum[2], sum[3]);
         }
         if (d == 0) {
-            if (sp.n > 1) sp.part_ml[r * sp.n + split] = float2{mm, ll};
-            else if (a.ml) a.ml[r] = float2{mm, ll};
+            if (sp.n > 1 || sp.counters) put2(reinterpret_cast<float*>(sp.part_ml + r * sp.n + split), mm, ll);
+            if (sp.n == 1 && a.ml) a.ml[r] = float2{mm, ll};
         }
     }
-}
-// Joins the splits of a row and head: one workgroup of D / 4 threads each; the statistics go to ml where weights are counted.
-template <int D>
-__global__ __launch_bounds__(64) void kv8_attn_join_kernel(Kv8Attn a, Kv8Split sp) {
-    const size_t r = blockIdx.x;
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < sp.n; i += 64) m = fmaxf(m, sp.part_ml[r * sp.n + i].x);
-    m = wave_max(m);
-    const float mu = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int i = threadIdx.x; i < sp.n; i += 64) { const float2 t = sp.part_ml[r * sp.n + i]; l = fmaf(t.y, __builtin_amdgcn_exp2f(t.x - mu), l); }
-    l = wave_sum(l);
-    if (threadIdx.x < D / 4) {
-        f4 sum = f4{0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < sp.n; ++i) {
-            const float e = __builtin_amdgcn_exp2f(sp.part_ml[r * sp.n + i].x - mu);
-            const f4 v = *reinterpret_cast<const f4*>(sp.part_o + (r * sp.n + i) * D + threadIdx.x * 4);
+    if (!sp.counters) return;
+    // The workgroup that finishes last for its columns joins the splits (in their order, whoever comes last) and counts the weights.
+    unsigned* counter = sp.counters + blockIdx.z * gridDim.y + hkv;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                 // this thread's parts and scores are where the others can see them
+    __syncthreads();
+    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)sp.n - 1;
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);        // as the next launch expects it
+    float* wgt = &so[0][0][0];                                       // [16][64] weights of the splits, then [16] maxima and [16] 1 / sums
+    for (int cn = w; cn < nv; cn += W) {
+        const int cc = blockIdx.z * 16 + cn;
+        const size_t r = out_row(cc);
+        const float2 ml = lane < sp.n ? get2(reinterpret_cast<const float*>(sp.part_ml + r * sp.n + lane)) : float2{-INFINITY, 0.f};
+        const float mm = wave_max(ml.x), e = __builtin_amdgcn_exp2f(ml.x - (mm == -INFINITY ? 0.f : mm)), ll = wave_sum(lane < sp.n ? ml.y * e : 0.f);
+        wgt[cn * 64 + lane] = e / ll;
+        if (lane == 0) { wgt[1024 + cn] = mm; wgt[1040 + cn] = 1.f / ll; if (a.ml) a.ml[r] = float2{mm, ll}; }
+    }
+    __syncthreads();
+    if (sp.n > 1)
+        for (int j = threadIdx.x; j < nv * (D / 2); j += 64 * W) {
+            const int cn = j / (D / 2), d = (j % (D / 2)) * 2, cc = blockIdx.z * 16 + cn;
+            const size_t r = out_row(cc);
+            const float* po = sp.part_o + r * sp.n * D + d;
+            float x = 0.f, y = 0.f;
+            for (int i0 = 0; i0 < sp.n; i0 += 8) {
+                float2 v[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sum[k] = fmaf(v[k], e, sum[k]);
+                for (int i = 0; i < 8; ++i) v[i] = get2(po + (size_t)min(i0 + i, sp.n - 1) * D);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float e = i0 + i < sp.n ? wgt[cn * 64 + i0 + i] : 0.f;
+                    x = i0 + i < sp.n ? fmaf(v[i].x, e, x) : x; y = i0 + i < sp.n ? fmaf(v[i].y, e, y) : y;
+                }
+            }
+            *reinterpret_cast<float2*>(a.out + r * D + d) = float2{x, y};
         }
+    if (sp.scores)                                                   // one row: columns are the heads of the group
+        for (int t2 = threadIdx.x * 2; t2 < a.mass_n; t2 += 128 * W) {
+            float x = 0.f, y = 0.f;
+            for (int g = 0; g < nv; ++g) {
+                const float2 s = get2(sp.scores + (size_t)(hkv * G + g) * sp.scores_ld + t2);
+                const float mm = wgt[1024 + g], il = wgt[1040 + g];
+                x = fmaf(__builtin_amdgcn_exp2f(s.x - mm), il, x); y = fmaf(__builtin_amdgcn_exp2f(s.y - mm), il, y);
+            }
+            const size_t at = (size_t)hkv * a.mass_ld + t2;
+            a.mass_out[at] = a.mass_in[at] + x;
+            if (t2 + 1 < a.mass_n) a.mass_out[at + 1] = a.mass_in[at + 1] + y;
+        }
+}
+// Joins many splits of a row and head, a workgroup each: 256 / (D / 4) groups of threads take the splits in turn.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_attn_join_kernel(Kv8Attn a, Kv8Split sp) {
+    constexpr int R = 256 / (D / 4);
+    __shared__ f4 part[R][D / 4];
+    const size_t r = blockIdx.x;
+    const int lane = threadIdx.x & 63, d = threadIdx.x % (D / 4), g = threadIdx.x / (D / 4);
+    const float2 ml = lane < sp.n ? sp.part_ml[r * sp.n + lane] : float2{-INFINITY, 0.f};
+    const float m = wave_max(ml.x), e = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m)), l = wave_sum(lane < sp.n ? ml.y * e : 0.f);
+    f4 sum = f4{0.f, 0.f, 0.f, 0.f};
+    for (int i = g; i < sp.n; i += R) {
+        const float ei = __shfl(e, i);
+        const f4 v = reinterpret_cast<const f4*>(sp.part_o + (r * sp.n + i) * D)[d];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] = fmaf(v[k], ei, sum[k]);
+    }
+    part[g][d] = sum;
+    __syncthreads();
+    if (threadIdx.x < D / 4) {
+        sum = part[0][d];
+#pragma unroll
+        for (int i = 1; i < R; ++i) sum += part[i][d];
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum[k] = sum[k] / l;
-        *reinterpret_cast<f4*>(a.out + r * D + threadIdx.x * 4) = sum;
+        reinterpret_cast<f4*>(a.out + r * D)[d] = sum;
     }
     if (threadIdx.x == 0 && a.ml) a.ml[r] = float2{m, l};
 }
@@ -529,27 +621,25 @@ __device__ __forceinline__ HF8x2 codes_f16(i4 q) {
     r.a = __builtin_bit_cast(hf8, lo); r.b = __builtin_bit_cast(hf8, hi);
     return r;
 }
-// hi and lo parts of eight f32; the empty asm keeps hi the rounding of the f32 value in both of its uses
-__device__ __forceinline__ void split_f16(const float (&x)[8], hf8& hi, hf8& lo) {
+// hi and lo parts of x[i] * f: hi the product cut to 11 bits, lo the rest of the exact product, rounded: together good to 2^-22 of it
+__device__ __forceinline__ void split_f16(const float* x, float f, hf8& hi, hf8& lo) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float v = x[i];
-        asm("" : "+v"(v));
-        hi[i] = (_Float16)v;
-        lo[i] = (_Float16)(v - (float)hi[i]);
+    for (int i = 0; i < 8; i += 2) {
+        const hf2 h = __builtin_bit_cast(hf2, __builtin_amdgcn_cvt_pkrtz(x[i] * f, x[i + 1] * f));
+        hi[i] = h[0]; hi[i + 1] = h[1];
+        lo[i] = (_Float16)fmaf(x[i], f, -(float)h[0]); lo[i + 1] = (_Float16)fmaf(x[i + 1], f, -(float)h[1]);
     }
 }
-// The B operand of q for one column: parts of dimensions (lane / 16) * D/4 + 8 st + j, st = 0 .. D/32 - 1.  Returns 1 / the power of two.
+// The B operand of q for one column: parts of dimensions 64 (st / 2) + 16 (lane / 16) + 8 (st % 2) + j, st = 0 .. D/32 - 1.  Returns 1 / the power of two.
 template <int D>
 __device__ __forceinline__ float load_q_f16(const float* q, bool valid, hf8 (&hi)[D / 32], hf8 (&lo)[D / 32]) {
-    float x[D / 4];
+    f4 x[D / 16];
+    load_q<D>(q, valid, x);
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-        const f4 v = valid ? reinterpret_cast<const f4*>(q)[i] : f4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { x[4 * i + j] = v[j]; const unsigned a = abs_bits(v[j]); m = a > m ? a : m; }
-    }
+        for (int j = 0; j < 4; ++j) { const unsigned u = abs_bits(x[i][j]); m = u > m ? u : m; }
     m = chunks_max_bits(m);
     const float amax = as_f(m);
     const bool fine = amax >= 0x1p-100f && m < 0x7F800000u;
@@ -559,8 +649,8 @@ __device__ __forceinline__ float load_q_f16(const float* q, bool valid, hf8 (&hi
     for (int st = 0; st < D / 32; ++st) {
         float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = fine ? x[8 * st + j] * up : 0.f;
-        split_f16(y, hi[st], lo[st]);
+        for (int j = 0; j < 8; ++j) y[j] = fine ? x[2 * st + j / 4][j % 4] : 0.f;
+        split_f16(y, up, hi[st], lo[st]);
     }
     return m >= 0x7F800000u ? as_f(0x7FC00000u) : ldexpf(1.f, e - 15);
 }
@@ -581,7 +671,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int bl
     const int G = c.H / c.Hkv, cols = a.M * G, col0 = blk * 64 * NC, wcol0 = col0 + w * 16 * NC;
     const int T = a.n_past + (min(col0 + 64 * NC, cols) - 1) / G + 1, tiles = (T + kKv8Tile - 1) / kKv8Tile;
     const int wrow0 = wcol0 / G, wrow1 = (min(wcol0 + 16 * NC, cols) - 1) / G;                             // rows this wave holds (none: wcol0 >= cols)
-    const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + 16 * (n >> 2) + (n & 3)) * D + ch * (D / 4);
+    const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + 16 * (n >> 2) + (n & 3)) * D + ch * 16;
     const int8_t* vb = c.v + (((size_t)hkv * c.n_blk + ch) * D + n) * 16;
     const float *ksb = c.ks + (size_t)hkv * c.n_blk + ch, *vsb = c.vs + (size_t)hkv * c.n_blk + ch;
 
@@ -591,7 +681,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int bl
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
             const int p = 4 * j + w;
-            const int8_t* src = p < 4 * (D / 64) ? kb + (size_t)t * (kKv8Tile * D) + 4 * (p / (D / 64)) * D + (p % (D / 64)) * 16 : vb + (size_t)t * (kKv8Tile * D) + (p - 4 * (D / 64)) * 256;
+            const int8_t* src = p < 4 * (D / 64) ? kb + (size_t)t * (kKv8Tile * D) + 4 * (p / (D / 64)) * D + (p % (D / 64)) * 64 : vb + (size_t)t * (kKv8Tile * D) + (p - 4 * (D / 64)) * 256;
             st[j] = *reinterpret_cast<const i4*>(src);
         }
     };
@@ -615,35 +705,56 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int bl
         const int col = wcol0 + 16 * k + n;
         const bool valid = col < cols;
         lim[k] = valid ? a.n_past + col / G : T - 1;
-        qf[k] = load_q_f16<D>(a.q + (valid ? (size_t)(col / G) * c.H + hkv * G + col % G : 0) * D + ch * (D / 4), valid, qh[k], ql[k]) * scale;
+        qf[k] = load_q_f16<D>(a.q + (valid ? (size_t)(col / G) * c.H + hkv * G + col % G : 0) * D + ch * 16, valid, qh[k], ql[k]) * scale;
         m[k] = -INFINITY; l[k] = 0.f; ref[k] = -1000;
 #pragma unroll
         for (int g = 0; g < NG; ++g) o[k][g] = f4{0.f, 0.f, 0.f, 0.f};
     }
     stage(0);
     float ks = ksb[0], vs = vsb[0];
+    asm("" : "+v"(ks), "+v"(vs));                                          // here, not in the loop, is where they are waited for
     __syncthreads();
-    for (int t = 0; t < tiles; ++t) {
-        const bool more = t + 1 < tiles;
+    // One tile.  `more` is a constant in each of its two uses: with a branch around the loads the compiler would wait for all of them wherever
+    // it waits for any.
+    auto step = [&](int t, auto more_) {
+        constexpr bool more = decltype(more_)::value;
         float ksn = 0.f, vsn = 0.f;
         if (more) { fetch(t + 1); ksn = ksb[(size_t)(t + 1) * 4]; vsn = vsb[(size_t)(t + 1) * 4]; }
         if (wcol0 < cols && t * kKv8Tile <= a.n_past + wrow1) {             // some row of this wave sees the tile
             const hf8* kf_ = frag + (size_t)(t & 1) * (KF + VF) * 64 + lane;
             const hf8* vf_ = kf_ + KF * 64;
+            // both products: the fragments of the next step are read while the present one's matrix instructions run, and 2 NC sums
+            // take turns, so that each finds its predecessor done
             f4 s[NC][4];
+            hf8 fr[2][2][2];                                               // [turn][group of the pair][step of the pair]
+            auto read_k = [&](int j) {                                     // pair j of groups x pair of steps
+                const int g = j / (ST / 2) * 2, i = j % (ST / 2) * 2;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
+                for (int x = 0; x < 2; ++x) { fr[j & 1][0][x] = kf_[(g * ST + i + x) * 64]; fr[j & 1][1][x] = kf_[((g + 1) * ST + i + x) * 64]; }
+            };
+            read_k(0);
 #pragma unroll
-                for (int k = 0; k < NC; ++k) s[k][g] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < ST; ++j) {
+                const int g = j / (ST / 2) * 2, i = j % (ST / 2) * 2;
+                if (j + 1 < ST) read_k(j + 1);
+                if (i == 0) {
 #pragma unroll
-                for (int i = 0; i < ST; ++i) {
-                    const hf8 kk = kf_[(g * ST + i) * 64];
+                    for (int k = 0; k < NC; ++k) s[k][g] = s[k][g + 1] = f4{0.f, 0.f, 0.f, 0.f};
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
 #pragma unroll
                     for (int k = 0; k < NC; ++k) {
-                        s[k][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[k][i], s[k][g], 0, 0, 0);
-                        s[k][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[k][i], s[k][g], 0, 0, 0);
+                        s[k][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[j & 1][0][x], qh[k][i + x], s[k][g], 0, 0, 0);
+                        s[k][g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[j & 1][1][x], qh[k][i + x], s[k][g + 1], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int k = 0; k < NC; ++k) {
+                        s[k][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[j & 1][0][x], ql[k][i + x], s[k][g], 0, 0, 0);
+                        s[k][g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[j & 1][1][x], ql[k][i + x], s[k][g + 1], 0, 0, 0);
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             hf8 ph[NC][2], pl[NC][2];
             const int pos = t * kKv8Tile + ch * 16;
@@ -683,28 +794,36 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int bl
                 l[k] += ls;
                 const float fac = ldexpf(vsu, 15 - ref[k]) + (as_f(wm) - as_f(wm));
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float x[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = p[8 * h + i] * fac;
-                    split_f16(x, ph[k][h], pl[k][h]);
-                }
+                for (int h = 0; h < 2; ++h) split_f16(p + 8 * h, fac, ph[k][h], pl[k][h]);
             }
+            auto read_v = [&](int j) {                                     // dimension pair j, both halves of the positions
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
+                for (int h = 0; h < 2; ++h) { fr[j & 1][0][h] = vf_[(4 * j + h) * 64]; fr[j & 1][1][h] = vf_[(4 * j + 2 + h) * 64]; }
+            };
+            read_v(0);
+#pragma unroll
+            for (int j = 0; j < NG / 2; ++j) {
+                if (j + 1 < NG / 2) read_v(j + 1);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const hf8 vv = vf_[(g * 2 + h) * 64];
 #pragma unroll
                     for (int k = 0; k < NC; ++k) {
-                        o[k][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[k][h], o[k][g], 0, 0, 0);
-                        o[k][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[k][h], o[k][g], 0, 0, 0);
+                        o[k][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[j & 1][0][h], ph[k][h], o[k][2 * j], 0, 0, 0);
+                        o[k][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[j & 1][1][h], ph[k][h], o[k][2 * j + 1], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int k = 0; k < NC; ++k) {
+                        o[k][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[j & 1][0][h], pl[k][h], o[k][2 * j], 0, 0, 0);
+                        o[k][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[j & 1][1][h], pl[k][h], o[k][2 * j + 1], 0, 0, 0);
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        if (more) { stage((t + 1) & 1); ks = ksn; vs = vsn; }
-        __syncthreads();
-    }
+        if (more) { stage((t + 1) & 1); ks = ksn; vs = vsn; __syncthreads(); }
+    };
+    for (int t = 0; t + 1 < tiles; ++t) step(t, std::true_type{});
+    step(tiles - 1, std::false_type{});
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
         const int col = wcol0 + 16 * k + n;
@@ -737,13 +856,13 @@ __global__ __launch_bounds__(256, 2) void kv8_mass_tile_kernel(Kv8Attn a, float 
     hf8 kk[TG][ST];
     float ks = 0.f;
     if (live) {
-        const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + (size_t)tile * kKv8Tile + 16 * (n >> 2) + (n & 3)) * D + ch * (D / 4);
+        const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + (size_t)tile * kKv8Tile + 16 * (n >> 2) + (n & 3)) * D + ch * 16;
         ks = c.ks[(size_t)hkv * c.n_blk + (size_t)tile * 4 + ch];
 #pragma unroll
         for (int g = 0; g < TG; ++g)
 #pragma unroll
             for (int kc = 0; kc < D / 64; ++kc) {
-                const HF8x2 h = codes_f16(*reinterpret_cast<const i4*>(kb + 4 * (g0 + g) * D + kc * 16));
+                const HF8x2 h = codes_f16(*reinterpret_cast<const i4*>(kb + 4 * (g0 + g) * D + kc * 64));
                 kk[g][2 * kc] = h.a; kk[g][2 * kc + 1] = h.b;
             }
     }
@@ -756,7 +875,7 @@ __global__ __launch_bounds__(256, 2) void kv8_mass_tile_kernel(Kv8Attn a, float 
         const bool valid = col < cols;
         const size_t r = valid ? (size_t)(col / G) * c.H + hkv * G + col % G : 0;
         hf8 hi[ST], lo[ST];
-        const float f = load_q_f16<D>(a.q + r * D + ch * (D / 4), valid, hi, lo) * scale;
+        const float f = load_q_f16<D>(a.q + r * D + ch * 16, valid, hi, lo) * scale;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < ST; ++i) { qs[(w * 2 * ST + i) * 64 + lane] = hi[i]; qs[(w * 2 * ST + ST + i) * 64 + lane] = lo[i]; }
@@ -871,11 +990,21 @@ hipError_t launch_kv8_attn_mass(const Kv8Attn& a, hipStream_t st) {
     KV8_BY_DIM(a.c.D, return mass_tile<kD>(a, st));
     return hipErrorInvalidValue;
 }
+template <int D, int W> static void attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t st) {
+    const dim3 grid(sp.n, a.c.Hkv, (a.M * (a.c.H / a.c.Hkv) + 15) / 16);
+    const float scale = kLog2e / sqrtf((float)D);
+    if (sp.stream) hipLaunchKernelGGL((kv8_attn_split_kernel<D, W, true>), grid, dim3(64 * W), 0, st, a, sp, scale);
+    else hipLaunchKernelGGL((kv8_attn_split_kernel<D, W, false>), grid, dim3(64 * W), 0, st, a, sp, scale);
+}
 hipError_t launch_kv8_attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t st) {
-    const int cols = a.M * (a.c.H / a.c.Hkv);
-    const dim3 grid(sp.n, a.c.Hkv, (cols + 15) / 16);
-    KV8_BY_DIM(a.c.D, hipLaunchKernelGGL(kv8_attn_split_kernel<kD>, grid, dim3(256), 0, st, a, sp, kLog2e / sqrtf((float)kD)));
-    if (sp.n > 1) KV8_BY_DIM(a.c.D, hipLaunchKernelGGL(kv8_attn_join_kernel<kD>, dim3(a.M * a.c.H), dim3(64), 0, st, a, sp));
+    switch (a.c.D) {
+        case 64: if (sp.waves == 8) attn_split<64, 8>(a, sp, st); else attn_split<64, 4>(a, sp, st); break;
+        case 128: if (sp.waves == 8) attn_split<128, 8>(a, sp, st); else if (sp.waves == 2) attn_split<128, 2>(a, sp, st); else attn_split<128, 4>(a, sp, st); break;
+        case 256: attn_split<256, 4>(a, sp, st); break;
+        default: return hipErrorInvalidValue;
+    }
+    if (sp.counters) return hipGetLastError();
+    if (sp.n > 1) KV8_BY_DIM(a.c.D, hipLaunchKernelGGL(kv8_attn_join_kernel<kD>, dim3(a.M * a.c.H), dim3(256), 0, st, a, sp));
     if (sp.scores) hipLaunchKernelGGL(kv8_mass_scores_kernel, dim3((a.mass_n + 1023) / 1024, a.c.Hkv), dim3(256), 0, st, a, sp);
     return hipGetLastError();
 }

@@ -8,6 +8,7 @@ namespace thk {
 static const int kKv8Block = 16;      // positions that share one K scale and one V scale per K/V head
 static const int kKv8Tile = 64;       // positions one step of the attention kernels takes: the cache is padded to whole tiles
 static const int kKv8SplitRows = 8192; // rows x splits whose parts the workspace holds
+static const int kKv8Counters = 8192;  // column groups x K/V heads that can be joined inside the launch
 static const int kKv8RowSlab = 2048;  // prompt rows one attention launch takes (sizes the per-row statistics)
 
 // Device memory of one cache.  n_blk = blocks per head, a multiple of 4 (whole tiles).
@@ -37,13 +38,16 @@ struct Kv8Attn {
     int mass_n;                       // entries per head that are written: all positions of the call, also those this slab's rows do not see yet
 };
 
-// Few rows over a long axis: the positions are cut into n parts of whole tiles, joined by a second launch when n > 1.
+// Few rows over a long axis: the positions are cut into n <= 64 parts of whole tiles.  With counters the last workgroup of a column group joins
+// the parts (and counts the weights), otherwise launches of their own do.
 struct Kv8Split {
-    int n;
+    int n, waves;                     // parts; waves of a workgroup, 4 or 8
+    bool stream;                      // the codes are read past the caches
     float* part_o;                    // [M H][n][D]
     float2* part_ml;                  // [M H][n]
     float* scores;                    // [H][scores_ld] base-2 scores of a single row, for the weight count; or null
     int64_t scores_ld;
+    unsigned* counters;               // one per column group and K/V head, zero between launches; or null
 };
 
 hipError_t launch_kv8_append(const Kv8View& c, const float* k, const float* v, int64_t pos, int64_t n, hipStream_t st);
