@@ -246,7 +246,7 @@ def test_garbage_behind_the_last_position(thk, ctx):
 
 
 @pytest.mark.parametrize("T,keep,sink,recent", [(1, 1, 0, 0), (40, 1, 0, 0), (40, 40, 0, 0), (64, 33, 4, 8), (500, 250, 4, 32), (300, 20, 10, 10), (300, 16, 16, 0), (1500, 1024, 0, 1),
-                                                (2500, 100, 1, 7), (257, 256, 0, 0)])
+                                                (2500, 100, 1, 7), (257, 256, 0, 0), (1024, 1000, 0, 0), (1025, 513, 3, 500), (4097, 700, 0, 64)])
 @pytest.mark.parametrize("Hkv,D", [(3, 128), (2, 64), (1, 256)])
 def test_evict(thk, ctx, Hkv, D, T, keep, sink, recent):
     rng = np.random.default_rng(T + keep + D)
@@ -265,6 +265,25 @@ def test_evict(thk, ctx, Hkv, D, T, keep, sink, recent):
     assert np.array_equal(p.read(0, T), p.ref.values(0, T))                         # the source stays
     dst.append(rows(rng, 5, Hkv, D), keep)                                          # and the destination goes on
     assert np.array_equal(dst.read(0, keep + 5), dst.ref.values(0, keep + 5))
+
+
+@pytest.mark.parametrize("T,keep", [(32768, 9000), (32769, 20011), (70001, 5), (140000, 139999)])
+def test_evict_long(thk, ctx, T, keep):
+    """The selection's other ranges: positions and weights only (the values of a few kept rows)."""
+    rng = np.random.default_rng(T)
+    kv, dst = thk.KvCache8(ctx, T, 2, 2, 64), thk.KvCache8(ctx, keep, 2, 2, 64)
+    mass = np.exp(rng.standard_normal((2, T)) * 3).astype(np.float32)
+    mass[1] = np.round(mass[1])
+    dm, mo, kept = ctx.from_numpy(mass), ctx.alloc(2 * keep * 4), ctx.alloc(2 * keep * 4)
+    kv.evict(dst, T, keep, 1, 2, dm, mo, kept)
+    for h in range(2):
+        mid = np.arange(1, T - 2)
+        heavy = mid[np.argsort(-mass[h, 1:T - 2].astype(np.float64), kind="stable")][:keep - 3]
+        exp = np.sort(np.concatenate([[0], heavy, [T - 2, T - 1]]))
+        assert np.array_equal(kept.download(np.int32, (2, keep))[h], exp)
+        assert np.array_equal(mo.download(np.float32, (2, keep))[h], mass[h][exp])
+    kv.close()
+    dst.close()
 
 
 def test_evict_odd_weights(thk, ctx):

@@ -53,7 +53,7 @@ extern "C" int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_
     if (!kv) return fail(ctx, THK_ERR_OOM, "thk_kv8_create: out of host memory");
     kv->ctx = ctx; kv->n_ctx = n_ctx;
     Kv8View& v = kv->view;
-    v.n_blk = (int)((n_ctx + kKv8Tile - 1) / kKv8Tile) * (kKv8Tile / kKv8Block);
+    v.n_blk = (int)((n_ctx + kKv8Pad - 1) / kKv8Pad) * (kKv8Pad / kKv8Block);
     v.H = (int)H; v.Hkv = (int)H_kv; v.D = (int)D;
     const size_t codes = (size_t)H_kv * v.n_blk * kKv8Block * D, scales = up256((size_t)H_kv * v.n_blk * 4), tail = (size_t)2 * H_kv * kKv8Block * D * 4;
     const size_t at = up256((size_t)2 * H_kv * sizeof(int2)), ml = (size_t)kKv8RowSlab * H * sizeof(float2);

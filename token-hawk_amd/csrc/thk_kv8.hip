@@ -60,20 +60,41 @@ __device__ void append_block(const Kv8View& c, int h, int b, const float* x, int
     float* tail = c.tail + ((size_t)(V ? c.Hkv : 0) + h) * (kKv8Block * D);
     int2* at = c.tail_at + (V ? c.Hkv : 0) + h;
     float xs[D / 16];
-    unsigned m = 0;
-    int held = 0;
-    float old = 0.f;
-    if (r0 > 0) { const int2 t = *at; held = t.x == b ? t.y : 0; old = *scale; }
+    const size_t ld = (size_t)c.Hkv * D;
+    const float* src = x + (p0 - pos) * (int64_t)ld + (size_t)h * D;        // row r of the block: src + r ld (the new rows only)
+    if (r0 == 0 && r1 == kKv8Block) {                                      // all rows are new: no choice, all loads at once
+        if (V) {
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-        const int r = el_row<D, V>(i), d = el_dim<D, V>(i);
-        float e = 0.f;
-        if (r >= r0 && r < r1) e = x[((size_t)(p0 + r - pos) * c.Hkv + h) * D + d];
-        else if (r < r0) e = r < held ? tail[r * D + d] : (float)codes[i] * old;
-        xs[i] = e;
-        const unsigned a = abs_bits(e);
-        m = a > m ? a : m;
+            for (int i = 0; i < D / 16; ++i) xs[i] = __builtin_nontemporal_load(src + (size_t)el_row<D, V>(0) * ld + i * ld + el_dim<D, V>(0));
+        } else {
+#pragma unroll
+            for (int i = 0; i < D / 16; i += 4) {
+                const f4 v = __builtin_nontemporal_load(reinterpret_cast<const f4*>(src + (size_t)el_row<D, V>(0) * ld + el_dim<D, V>(0) + i));
+                xs[i] = v[0]; xs[i + 1] = v[1]; xs[i + 2] = v[2]; xs[i + 3] = v[3];
+            }
+        }
+    } else {                                                               // every source is read (rows out of reach: the nearest that exists), then one is taken
+        const int2 t = *at;
+        const float old = *scale;
+        float xn[D / 16], xt[D / 16];
+        int8_t xc[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const int r = el_row<D, V>(i), d = el_dim<D, V>(i);
+            xn[i] = src[(size_t)min(max(r, r0), r1 - 1) * ld + d];
+            xt[i] = tail[r * D + d];
+            xc[i] = codes[i];
+        }
+        const int held = t.x == b ? t.y : 0;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const int r = el_row<D, V>(i);
+            xs[i] = r >= r1 ? 0.f : r >= r0 ? xn[i] : r < held ? xt[i] : (float)xc[i] * old;
+        }
     }
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) { const unsigned u = abs_bits(xs[i]); m = u > m ? u : m; }
     const Quant qz = quant_of(block_max_u32(m, sm));
     unsigned q[D / 16];
 #pragma unroll
@@ -140,54 +161,120 @@ __device__ __forceinline__ unsigned block_scan_1024(unsigned v, unsigned* sm, un
     *total = all;
     return before + s - v;
 }
-// One workgroup per K/V head: the n_keep - n_sink - n_recent heaviest of the middle positions by radix selection (four passes of 8 bits,
-// histograms in LDS), ties to the lowest position, then the kept positions in ascending order.
+// One workgroup per K/V head: the n_keep - n_sink - n_recent heaviest of the middle positions by radix selection (11, 11 and 10 bits of the
+// keys, histograms in LDS), ties to the lowest position, then the kept positions in ascending order.  Thread t has positions t + 1024 i; with
+// N > 0 (T <= 1024 N) their keys stay in registers, else every pass reads the weights again.  Which positions stay is written down as one
+// 64-bit ballot per 64 positions, whose bit counts, summed up, say where each wave's kept positions go; N = 0 does that 64 times 1024
+// positions at a time.
+template <int N>
 __global__ __launch_bounds__(1024) void kv8_select_kernel(int T, int n_keep, int n_sink, int n_recent, const float* __restrict__ mass_in, int64_t ld_in,
                                                           float* __restrict__ mass_out, int64_t ld_out, int32_t* __restrict__ kept) {
-    __shared__ unsigned hist[256], sm[16], pick[2];
-    const int h = blockIdx.x, tid = threadIdx.x, lo = n_sink, hi = T - n_recent;
+    constexpr int C = N > 0 ? N : 64;                                      // positions of a thread in one sweep
+    __shared__ unsigned hist[2][2048], sm[16], pick[2];
+    __shared__ unsigned cnt[1024];                                         // [64 slices of 1024][16 waves]
+    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, lo = n_sink, hi = T - n_recent;
     const float* mass = mass_in + (size_t)h * ld_in;
     unsigned need = (unsigned)(n_keep - n_sink - n_recent), prefix = 0;     // of the positions whose key starts with prefix, the `need` heaviest stay
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+    unsigned keys[C];
+    auto key_at = [&](int t) { return mass_key(mass[t < T ? t : T - 1]); };
+    if (N > 0) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) keys[i] = key_at(i * 1024 + tid);
+    }
+    int shift = 32;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int bits = pass < 2 ? 11 : 10, prev = shift;
+        shift -= bits;
+        const unsigned mask = (1u << bits) - 1;
+        hist[0][tid] = hist[0][tid + 1024] = hist[1][tid] = hist[1][tid + 1024] = 0;
         __syncthreads();
-        for (int t = lo + tid; t < hi; t += 1024) {
-            const unsigned key = mass_key(mass[t]);
-            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);    // integer: the order changes nothing
+        auto count = [&](int t, unsigned key) {
+            if (t >= lo && t < hi && (pass == 0 || (key >> prev) == prefix)) atomicAdd(&hist[w & 1][(key >> shift) & mask], 1u);    // integers: the order changes nothing
+        };
+        if (N > 0) {
+#pragma unroll
+            for (int i = 0; i < C; ++i) count(i * 1024 + tid, keys[i]);
+        } else {
+            for (int t = tid; t < T; t += 1024) count(t, key_at(t));
         }
         __syncthreads();
         unsigned total;
-        const unsigned mine = tid < 256 ? hist[255 - tid] : 0u;              // thread i: the bucket of digit 255 - i
-        const unsigned above = block_scan_1024(mine, sm, &total);
-        if (tid < 256 && above < need && need <= above + mine) { pick[0] = 255u - tid; pick[1] = need - above; }
-        if (tid == 0 && need == 0) { pick[0] = 255u; pick[1] = 0u; }
+        const int top = (int)mask - 2 * tid;                               // thread i: buckets of digits top and top - 1, heaviest first
+        const unsigned c0 = top >= 0 ? hist[0][top] + hist[1][top] : 0u, c1 = top >= 1 ? hist[0][top - 1] + hist[1][top - 1] : 0u;
+        const unsigned above = block_scan_1024(c0 + c1, sm, &total);
+        if (above < need && need <= above + c0) { pick[0] = (unsigned)top; pick[1] = need - above; }
+        else if (above + c0 < need && need <= above + c0 + c1) { pick[0] = (unsigned)top - 1; pick[1] = need - above - c0; }
+        if (tid == 0 && need == 0) { pick[0] = mask; pick[1] = 0; }
         __syncthreads();
-        prefix = (prefix << 8) | pick[0];
+        prefix = (prefix << bits) | pick[0];
         need = pick[1];
         __syncthreads();
     }
-    // every thread takes a contiguous share of the positions: heavier ones stay, of those equal to the threshold the first `need`
-    const int per = (T + 1023) / 1024, t0 = tid * per < T ? tid * per : T, t1 = t0 + per < T ? t0 + per : T;
-    unsigned eq = 0, dummy;
-    for (int t = t0; t < t1; ++t) if (t >= lo && t < hi) eq += mass_key(mass[t]) == prefix;
-    unsigned rank = block_scan_1024(eq, sm, &dummy);
-    unsigned cnt = 0, r = rank;
-    for (int t = t0; t < t1; ++t) {
-        if (t < lo || t >= hi) { ++cnt; continue; }
-        const unsigned key = mass_key(mass[t]);
-        cnt += key > prefix || (key == prefix && r < need);
-        r += key == prefix;
-    }
-    unsigned at = block_scan_1024(cnt, sm, &dummy);
-    r = rank;
-    for (int t = t0; t < t1; ++t) {
-        bool stay = t < lo || t >= hi;
-        if (!stay) {
-            const unsigned key = mass_key(mass[t]);
-            stay = key > prefix || (key == prefix && r < need);
-            r += key == prefix;
+    // of the positions equal to the threshold the first `need` stay: a sweep for their ranks, a sweep for the places of those that stay
+    unsigned eq_before = 0, kept_before = 0, all;
+#pragma unroll 1
+    for (int t0 = 0; t0 < T; t0 += C * 1024) {
+        if (N == 0) {
+#pragma unroll 1
+            for (int i = 0; i < C; ++i) {
+                const int t = t0 + i * 1024 + tid;
+                const unsigned long long b = __ballot(t >= lo && t < hi && key_at(t) == prefix);
+                if (lane == 0) cnt[i * 16 + w] = (unsigned)__popcll(b);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const int t = t0 + i * 1024 + tid;
+                const unsigned long long b = __ballot(t >= lo && t < hi && keys[i] == prefix);
+                if (lane == 0) cnt[i * 16 + w] = (unsigned)__popcll(b);
+            }
         }
-        if (stay) { kept[(size_t)h * n_keep + at] = t; if (mass_out) mass_out[(size_t)h * ld_out + at] = mass[t]; ++at; }
+        __syncthreads();
+        const unsigned eq = block_scan_1024(tid < C * 16 ? cnt[tid] : 0u, sm, &all) + eq_before;
+        eq_before += all;
+        __syncthreads();
+        if (tid < C * 16) cnt[tid] = eq;
+        __syncthreads();
+        unsigned long long mine = 0;                                       // bit i: this thread's position i stays
+        auto decide = [&](int i, unsigned key) {
+            const int t = t0 + i * 1024 + tid;
+            const bool mid = t >= lo && t < hi, same = mid && key == prefix;
+            const unsigned long long b = __ballot(same);
+            const bool stay = t < T && (!mid || key > prefix || (same && cnt[i * 16 + w] + (unsigned)__popcll(b & ((1ull << lane) - 1)) < need));
+            mine |= (unsigned long long)stay << i;
+        };
+        if (N == 0) {
+#pragma unroll 1
+            for (int i = 0; i < C; ++i) decide(i, key_at(t0 + i * 1024 + tid));
+        } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i) decide(i, keys[i]);
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int i = 0; i < C; ++i) {
+            const unsigned long long b = __ballot(mine >> i & 1);
+            if (lane == 0) cnt[i * 16 + w] = (unsigned)__popcll(b);
+        }
+        __syncthreads();
+        const unsigned at0 = block_scan_1024(tid < C * 16 ? cnt[tid] : 0u, sm, &all) + kept_before;
+        kept_before += all;
+        __syncthreads();
+        if (tid < C * 16) cnt[tid] = at0;
+        __syncthreads();
+#pragma unroll 1
+        for (int i = 0; i < C; ++i) {
+            const bool stay = mine >> i & 1;
+            const unsigned long long b = __ballot(stay);
+            if (stay) {
+                const int t = t0 + i * 1024 + tid;
+                const unsigned at = cnt[i * 16 + w] + (unsigned)__popcll(b & ((1ull << lane) - 1));
+                kept[(size_t)h * n_keep + at] = t;
+                if (mass_out) mass_out[(size_t)h * ld_out + at] = mass[t];
+            }
+        }
+        __syncthreads();
     }
 }
 // One workgroup per destination block, head and K | V: gathers the 16 kept rows as values and quantises them anew.  Sixteen rows that were
@@ -201,18 +288,22 @@ __device__ __forceinline__ void move_body(const Kv8View& s, const Kv8View& d, in
     const int8_t* from = (V ? s.v : s.k) + (size_t)h * s.n_blk * (kKv8Block * D);
     const float* sc = (V ? s.vs : s.ks) + (size_t)h * s.n_blk;
     const size_t hb = (size_t)h * d.n_blk + b;
-    float xs[D / 16];
+    float xs[D / 16], sc_[D / 16];
     unsigned q[D / 16], m = 0;
+    int8_t code[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {                                     // rows behind the last kept one read position 0: all loads at once
+        const int p = max(src[el_row<D, V>(i)], 0), dim = el_dim<D, V>(i);
+        code[i] = V ? from[((size_t)(p >> 4) * D + dim) * 16 + (p & 15)] : from[(size_t)p * D + dim];
+        sc_[i] = sc[p >> 4];
+    }
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
-        const int p = src[el_row<D, V>(i)], dim = el_dim<D, V>(i);
-        int code = 0;
-        float scale = 0.f;
-        if (p >= 0) { code = V ? from[((size_t)(p >> 4) * D + dim) * 16 + (p & 15)] : from[(size_t)p * D + dim]; scale = sc[p >> 4]; }
-        q[i] = (unsigned)code & 0xFFu;
-        xs[i] = (float)code * scale;
-        const unsigned a = abs_bits(xs[i]);
-        m = a > m ? a : m;
+        const bool in = src[el_row<D, V>(i)] >= 0;
+        q[i] = in ? (unsigned)code[i] & 0xFFu : 0u;
+        xs[i] = in ? (float)code[i] * sc_[i] : 0.f;
+        const unsigned u = abs_bits(xs[i]);
+        m = u > m ? u : m;
     }
     const Quant qz = quant_of(block_max_u32(m, sm));
     float scale = qz.scale;
@@ -761,7 +852,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int bl
             const bool edge = t * kKv8Tile + kKv8Tile - 1 > a.n_past + wrow0;
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
-                const float kf = qf[k] * ks;
+                // a block nobody sees has only -inf: its own factor may be NaN; and zero times -inf would be
+                const float kf = pos <= lim[k] && qf[k] * ks != 0.f ? qf[k] * ks : 1.f;
                 if (edge) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[k][i >> 2][i & 3] = pos + i <= lim[k] ? s[k][i >> 2][i & 3] : -INFINITY;
@@ -769,13 +861,12 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int bl
                 float top = s[k][0][0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) top = fmaxf(top, s[k][i >> 2][i & 3]);
-                top = pos <= lim[k] ? top * kf : -INFINITY;                // kf >= 0, but 0 * -inf is NaN
+                top *= kf;
                 const float mn = fmaxf(m[k], chunks_max(top)), mu = mn == -INFINITY ? 0.f : mn;
                 float p[16], ls = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     p[i] = __builtin_amdgcn_exp2f(fmaf(s[k][i >> 2][i & 3], kf, -mu));
-                    if (edge) p[i] = pos + i <= lim[k] ? p[i] : 0.f;
                     ls += p[i];
                 }
                 const float vsu = pos <= lim[k] ? vs : 0.f;
@@ -946,7 +1037,12 @@ hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_ou
 }
 hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recent, const float* mass_in, int64_t ld_in, float* mass_out, int64_t ld_out, int32_t* kept,
                              hipStream_t st) {
-    hipLaunchKernelGGL(kv8_select_kernel, dim3(Hkv), dim3(1024), 0, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept);
+#define KV8_SELECT(N) hipLaunchKernelGGL(kv8_select_kernel<N>, dim3(Hkv), dim3(1024), 0, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept)
+    if (T <= 1024) KV8_SELECT(1);
+    else if (T <= 4096) KV8_SELECT(4);
+    else if (T <= 32768) KV8_SELECT(32);
+    else KV8_SELECT(0);
+#undef KV8_SELECT
     return hipGetLastError();
 }
 hipError_t launch_kv8_move(const Kv8View& src, const Kv8View& dst, int n_keep, const int32_t* kept, hipStream_t st) {

@@ -6,12 +6,13 @@
 namespace thk {
 
 static const int kKv8Block = 16;      // positions that share one K scale and one V scale per K/V head
-static const int kKv8Tile = 64;       // positions one step of the attention kernels takes: the cache is padded to whole tiles
+static const int kKv8Tile = 64;       // positions one step of the split attention kernel takes
+static const int kKv8Pad = 128;       // a cache holds whole multiples of this many positions: no kernel's step reads behind it
 static const int kKv8SplitRows = 8192; // rows x splits whose parts the workspace holds
 static const int kKv8Counters = 8192;  // column groups x K/V heads that can be joined inside the launch
 static const int kKv8RowSlab = 2048;  // prompt rows one attention launch takes (sizes the per-row statistics)
 
-// Device memory of one cache.  n_blk = blocks per head, a multiple of 4 (whole tiles).
+// Device memory of one cache.  n_blk = blocks per head, a multiple of 8 (kKv8Pad).
 //   k    int8 [Hkv][n_blk][16][D]    codes, row-major: a position's D codes are contiguous
 //   v    int8 [Hkv][n_blk][D][16]    codes, transposed inside the block: the 16 positions of one dimension are contiguous, which is
 //                                    the operand chunk of one lane when positions are the summed axis of a matrix instruction
