@@ -127,10 +127,20 @@ __device__ __forceinline__ void read_body(const Kv8View& c, int64_t pos, int64_t
     const size_t hb = (size_t)h * c.n_blk + b;
     const int8_t* codes = (V ? c.v : c.k) + hb * (kKv8Block * D) + code_at<D, V>();
     const float s = (V ? c.vs : c.ks)[hb];
+    float xs[D / 16];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-        const int64_t p = (int64_t)b * kKv8Block + el_row<D, V>(i);
-        if (p >= pos && p < pos + n) out[((size_t)(p - pos) * c.Hkv + h) * D + el_dim<D, V>(i)] = (float)codes[i] * s;
+    for (int i = 0; i < D / 16; ++i) xs[i] = (float)codes[i] * s;
+    const int64_t p0 = (int64_t)b * kKv8Block - pos, ld = (int64_t)c.Hkv * D;
+    float* to = out + p0 * ld + (int64_t)h * D + el_dim<D, V>(0);          // row r of the block: to + r ld
+    if (V) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const int r = el_row<D, V>(i);
+            if (p0 + r >= 0 && p0 + r < n) to[r * ld] = xs[i];
+        }
+    } else if (p0 + el_row<D, V>(0) >= 0 && p0 + el_row<D, V>(0) < n) {
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 4) *reinterpret_cast<f4*>(to + el_row<D, V>(0) * ld + i) = f4{xs[i], xs[i + 1], xs[i + 2], xs[i + 3]};
     }
 }
 template <int D>
@@ -166,20 +176,21 @@ __device__ __forceinline__ unsigned block_scan_1024(unsigned v, unsigned* sm, un
 // N > 0 (T <= 1024 N) their keys stay in registers, else every pass reads the weights again.  Which positions stay is written down as one
 // 64-bit ballot per 64 positions, whose bit counts, summed up, say where each wave's kept positions go; N = 0 does that 64 times 1024
 // positions at a time.
+static const int kKv8Hist = 4;
 template <int N>
 __global__ __launch_bounds__(1024) void kv8_select_kernel(int T, int n_keep, int n_sink, int n_recent, const float* __restrict__ mass_in, int64_t ld_in,
                                                           float* __restrict__ mass_out, int64_t ld_out, int32_t* __restrict__ kept) {
     constexpr int C = N > 0 ? N : 64;                                      // positions of a thread in one sweep
-    __shared__ unsigned hist[2][2048], sm[16], pick[2];
+    __shared__ unsigned hist[kKv8Hist][2048], sm[16], pick[2];            // copies by lane: the weights' leading bits take few values
     __shared__ unsigned cnt[1024];                                         // [64 slices of 1024][16 waves]
     const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, lo = n_sink, hi = T - n_recent;
     const float* mass = mass_in + (size_t)h * ld_in;
     unsigned need = (unsigned)(n_keep - n_sink - n_recent), prefix = 0;     // of the positions whose key starts with prefix, the `need` heaviest stay
-    unsigned keys[C];
+    float x[C];                                                            // the weights themselves: a key is three operations, a second read is not
     auto key_at = [&](int t) { return mass_key(mass[t < T ? t : T - 1]); };
     if (N > 0) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) keys[i] = key_at(i * 1024 + tid);
+        for (int i = 0; i < C; ++i) x[i] = mass[min(i * 1024 + tid, T - 1)];
     }
     int shift = 32;
 #pragma unroll 1
@@ -187,21 +198,26 @@ __global__ __launch_bounds__(1024) void kv8_select_kernel(int T, int n_keep, int
         const int bits = pass < 2 ? 11 : 10, prev = shift;
         shift -= bits;
         const unsigned mask = (1u << bits) - 1;
-        hist[0][tid] = hist[0][tid + 1024] = hist[1][tid] = hist[1][tid + 1024] = 0;
+#pragma unroll
+        for (int i = 0; i < kKv8Hist; ++i) hist[i][tid] = hist[i][tid + 1024] = 0;
         __syncthreads();
         auto count = [&](int t, unsigned key) {
-            if (t >= lo && t < hi && (pass == 0 || (key >> prev) == prefix)) atomicAdd(&hist[w & 1][(key >> shift) & mask], 1u);    // integers: the order changes nothing
+            if (t >= lo && t < hi && (pass == 0 || (key >> prev) == prefix)) atomicAdd(&hist[lane % kKv8Hist][(key >> shift) & mask], 1u);    // integers: the order changes nothing
         };
         if (N > 0) {
 #pragma unroll
-            for (int i = 0; i < C; ++i) count(i * 1024 + tid, keys[i]);
+            for (int i = 0; i < C; ++i) count(i * 1024 + tid, mass_key(x[i]));
         } else {
             for (int t = tid; t < T; t += 1024) count(t, key_at(t));
         }
         __syncthreads();
         unsigned total;
         const int top = (int)mask - 2 * tid;                               // thread i: buckets of digits top and top - 1, heaviest first
-        const unsigned c0 = top >= 0 ? hist[0][top] + hist[1][top] : 0u, c1 = top >= 1 ? hist[0][top - 1] + hist[1][top - 1] : 0u;
+        unsigned c0 = 0, c1 = 0;
+        if (top > 0) {
+#pragma unroll
+            for (int i = 0; i < kKv8Hist; ++i) { c0 += hist[i][top]; c1 += hist[i][top - 1]; }
+        }
         const unsigned above = block_scan_1024(c0 + c1, sm, &total);
         if (above < need && need <= above + c0) { pick[0] = (unsigned)top; pick[1] = need - above; }
         else if (above + c0 < need && need <= above + c0 + c1) { pick[0] = (unsigned)top - 1; pick[1] = need - above - c0; }
@@ -226,7 +242,7 @@ __global__ __launch_bounds__(1024) void kv8_select_kernel(int T, int n_keep, int
 #pragma unroll
             for (int i = 0; i < C; ++i) {
                 const int t = t0 + i * 1024 + tid;
-                const unsigned long long b = __ballot(t >= lo && t < hi && keys[i] == prefix);
+                const unsigned long long b = __ballot(t >= lo && t < hi && mass_key(x[i]) == prefix);
                 if (lane == 0) cnt[i * 16 + w] = (unsigned)__popcll(b);
             }
         }
@@ -249,7 +265,7 @@ __global__ __launch_bounds__(1024) void kv8_select_kernel(int T, int n_keep, int
             for (int i = 0; i < C; ++i) decide(i, key_at(t0 + i * 1024 + tid));
         } else {
 #pragma unroll
-            for (int i = 0; i < C; ++i) decide(i, keys[i]);
+            for (int i = 0; i < C; ++i) decide(i, mass_key(x[i]));
         }
         __syncthreads();
 #pragma unroll 1
@@ -263,18 +279,68 @@ __global__ __launch_bounds__(1024) void kv8_select_kernel(int T, int n_keep, int
         __syncthreads();
         if (tid < C * 16) cnt[tid] = at0;
         __syncthreads();
-#pragma unroll 1
-        for (int i = 0; i < C; ++i) {
+        auto put = [&](int i, float v) {
             const bool stay = mine >> i & 1;
             const unsigned long long b = __ballot(stay);
             if (stay) {
-                const int t = t0 + i * 1024 + tid;
                 const unsigned at = cnt[i * 16 + w] + (unsigned)__popcll(b & ((1ull << lane) - 1));
-                kept[(size_t)h * n_keep + at] = t;
-                if (mass_out) mass_out[(size_t)h * ld_out + at] = mass[t];
+                kept[(size_t)h * n_keep + at] = t0 + i * 1024 + tid;
+                if (mass_out) mass_out[(size_t)h * ld_out + at] = v;
             }
+        };
+        if (N == 0) {
+#pragma unroll 1
+            for (int i = 0; i < C; ++i) put(i, mass[min(t0 + i * 1024 + tid, T - 1)]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i) put(i, x[i]);
         }
         __syncthreads();
+    }
+}
+// Few positions (T <= 64 N): one wave per head holds all keys, N a lane, and finds the threshold bit by bit with ballots - no LDS, no barrier.
+template <int N>
+__global__ __launch_bounds__(64) void kv8_select_wave_kernel(int T, int n_keep, int n_sink, int n_recent, const float* __restrict__ mass_in, int64_t ld_in,
+                                                             float* __restrict__ mass_out, int64_t ld_out, int32_t* __restrict__ kept) {
+    const int h = blockIdx.x, lane = threadIdx.x, lo = n_sink, hi = T - n_recent;
+    const float* mass = mass_in + (size_t)h * ld_in;
+    const int need = n_keep - n_sink - n_recent;
+    float x[N];
+    unsigned keys[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = mass[min(i * 64 + lane, T - 1)];
+    unsigned long long mid[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) { keys[i] = mass_key(x[i]); const int t = i * 64 + lane; mid[i] = __ballot(t >= lo && t < hi); }
+    unsigned thr = 0;                                                      // the largest value that `need` keys of the middle reach, two bits a turn
+#pragma unroll 1
+    for (int b = 30; b >= 0; b -= 2) {
+        int c[3] = {0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) c[j] += (int)__popcll(__ballot(keys[i] >= (thr | (unsigned)(j + 1) << b)) & mid[i]);
+        thr |= (c[2] >= need ? 3u : c[1] >= need ? 2u : c[0] >= need ? 1u : 0u) << b;
+    }
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) above += (int)__popcll(__ballot(keys[i] > thr) & mid[i]);
+    int ties = need - above, at = 0;                                       // of those equal to it the first `ties` stay
+    const unsigned long long below = (1ull << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int t = i * 64 + lane;
+        const unsigned long long same = __ballot(keys[i] == thr) & mid[i];
+        const bool in = mid[i] >> lane & 1;
+        const bool stay = t < T && (!in || (need > 0 && (keys[i] > thr || (keys[i] == thr && (int)__popcll(same & below) < ties))));
+        ties -= (int)__popcll(same);
+        const unsigned long long s = __ballot(stay);
+        if (stay) {
+            const size_t to = (size_t)(at + (int)__popcll(s & below));
+            kept[(size_t)h * n_keep + to] = t;
+            if (mass_out) mass_out[(size_t)h * ld_out + to] = x[i];
+        }
+        at += (int)__popcll(s);
     }
 }
 // One workgroup per destination block, head and K | V: gathers the 16 kept rows as values and quantises them anew.  Sixteen rows that were
@@ -928,85 +994,73 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int bl
 }
 
 // ---------------------------------------------------------------- weight count of many rows
-// mass_out = mass_in + sum over the columns of exp2(s - m) / l: a wave keeps the K fragments of 16 TG positions in registers and walks the
-// columns, whose q parts the workgroup stages 64 at a time; columns sum in a fixed order.
-template <int D, int TG>
-__global__ __launch_bounds__(256, 2) void kv8_mass_tile_kernel(Kv8Attn a, float scale) {
-    constexpr int ST = D / 32;
-    extern __shared__ __align__(16) char smem[];
-    hf8* qs = reinterpret_cast<hf8*>(smem);                                // [4 column groups][2 parts][ST][64]
-    float2* stat = reinterpret_cast<float2*>(qs + 4 * 2 * ST * 64);        // [64]: q factor / maximum
-    float* rl = reinterpret_cast<float*>(stat + 64);                       // [64]: 1 / sum
+// mass_out = mass_in + sum over the columns of exp2(s - m) / l.  A workgroup takes 64 positions; its W waves share the columns, 16 at a time
+// in turn, each with the K fragments of all 64 positions in registers and the next columns' q on the way; the waves' sums are added in a
+// fixed order.
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_mass_tile_kernel(Kv8Attn a, float scale) {
+    constexpr int KC = D / 64;
+    __shared__ float part[W][64];
     const Kv8View& c = a.c;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, ch = lane >> 4, hkv = blockIdx.y, G = c.H / c.Hkv, cols = a.M * G;
-    // wave's positions: TG == 4: tile 4 blockIdx.x + w, lane chunk ch and score 4 g + i is position 16 ch + 4 g + i of it;
-    // TG == 1: group w of tile blockIdx.x: position 16 ch + 4 w + i
-    const int tile = TG == 4 ? blockIdx.x * 4 + w : blockIdx.x, g0 = TG == 4 ? 0 : w, first = (TG == 4 ? blockIdx.x * 4 : blockIdx.x) * kKv8Tile;
-    const bool live = tile * kKv8Tile < a.n_past + a.M;
-    const int pos = tile * kKv8Tile + ch * 16 + 4 * g0;
-    hf8 kk[TG][ST];
-    float ks = 0.f;
-    if (live) {
-        const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + (size_t)tile * kKv8Tile + 16 * (n >> 2) + (n & 3)) * D + ch * 16;
-        ks = c.ks[(size_t)hkv * c.n_blk + (size_t)tile * 4 + ch];
+    const int tile = blockIdx.x, pos = tile * kKv8Tile + ch * 16;          // lane chunk ch, score i: position pos + i
+    const int row0 = max(tile * kKv8Tile - a.n_past, 0);                   // the first row that sees a position of this tile
+    const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + (size_t)tile * kKv8Tile + 16 * (n >> 2) + (n & 3)) * D + ch * 16;
+    i4 kr[4][KC];
 #pragma unroll
-        for (int g = 0; g < TG; ++g)
+    for (int g = 0; g < 4; ++g)
 #pragma unroll
-            for (int kc = 0; kc < D / 64; ++kc) {
-                const HF8x2 h = codes_f16(*reinterpret_cast<const i4*>(kb + 4 * (g0 + g) * D + kc * 64));
-                kk[g][2 * kc] = h.a; kk[g][2 * kc + 1] = h.b;
-            }
-    }
-    float sum[TG * 4];
+        for (int kc = 0; kc < KC; ++kc) kr[g][kc] = *reinterpret_cast<const i4*>(kb + 4 * g * D + kc * 64);
+    const float ks = c.ks[(size_t)hkv * c.n_blk + (size_t)tile * 4 + ch];
+    float sum[16];
 #pragma unroll
-    for (int i = 0; i < TG * 4; ++i) sum[i] = 0.f;
-    const int row0 = max(first - a.n_past, 0);                             // the first row that sees a position of this workgroup
-    for (int c0 = row0 * G / 64 * 64; c0 < cols; c0 += 64) {
-        const int col = c0 + w * 16 + n;
-        const bool valid = col < cols;
-        const size_t r = valid ? (size_t)(col / G) * c.H + hkv * G + col % G : 0;
-        hf8 hi[ST], lo[ST];
-        const float f = load_q_f16<D>(a.q + r * D + ch * 16, valid, hi, lo) * scale;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < ST; ++i) { qs[(w * 2 * ST + i) * 64 + lane] = hi[i]; qs[(w * 2 * ST + ST + i) * 64 + lane] = lo[i]; }
-        if (ch == 0) { const float2 t = valid ? a.ml[r] : float2{0.f, 1.f}; stat[w * 16 + n] = float2{f, t.x}; rl[w * 16 + n] = valid ? 1.f / t.y : 0.f; }
-        __syncthreads();
-        if (!live) continue;
+    for (int i = 0; i < 16; ++i) sum[i] = 0.f;
+    f4 x[D / 16];
+    float2 ml;
+    auto load = [&](int c0) {                                              // columns c0 + n; behind the last one the last one again
+        const int col = min(c0 + n, cols - 1), row = col / G;
+        const size_t r = (size_t)row * c.H + hkv * G + (col - row * G);
+        load_q<D>(a.q + r * D + ch * 16, true, x);
+        ml = a.ml[r];
+    };
+    int c0 = row0 * G / 16 * 16 + w * 16;
+    if (c0 < cols) load(c0);
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-            if (c0 + q * 16 >= cols) break;
-            const float2 sf = stat[q * 16 + n];
-            const float inv = rl[q * 16 + n], kf = sf.x * ks;
-            const int lim = a.n_past + min((c0 + q * 16 + n) / G, a.M - 1);
-            const hf8* qq = qs + (q * 2 * ST) * 64 + lane;
-            f4 s[TG];
+    for (; c0 < cols; c0 += 16 * W) {
+        i4 qd[3][KC];
+        const float qf = q_digits<D>(x, qd) * scale, top = ml.x, inv = 1.f / ml.y;
+        load(min(c0 + 16 * W, cols - 1));                                      // without a branch: the next ones, or any
+        const int row = min(c0 + n, cols - 1) / G, lim = c0 + n < cols ? a.n_past + row : -1;
+        const float kf = pos <= lim && qf * ks != 0.f ? qf * ks : 1.f;     // a block this column does not see: no factor that could be NaN
 #pragma unroll
-            for (int g = 0; g < TG; ++g) s[g] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int g = 0; g < 4; ++g) {
+            i4 acc[3];
 #pragma unroll
-            for (int i = 0; i < ST; ++i) {
-                const hf8 qh = qq[i * 64], ql = qq[(ST + i) * 64];
+            for (int d = 0; d < 3; ++d) {
+                acc[d] = i4{0, 0, 0, 0};
 #pragma unroll
-                for (int g = 0; g < TG; ++g) {
-                    s[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[g][i], qh, s[g], 0, 0, 0);
-                    s[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[g][i], ql, s[g], 0, 0, 0);
-                }
+                for (int kc = 0; kc < KC; ++kc) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[g][kc], qd[d][kc], acc[d], 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < TG * 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], kf, -sf.y)) * inv;
-                sum[i] += pos + i <= lim && c0 + q * 16 + n < cols ? p : 0.f;
+            for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(join_digits(acc[2][i], acc[1][i], acc[0][i]), kf, -top)) * inv;
+                sum[4 * g + i] += pos + 4 * g + i <= lim ? p : 0.f;
             }
         }
     }
-    if (!live) return;
 #pragma unroll
-    for (int i = 0; i < TG * 4; ++i) {
+    for (int i = 0; i < 16; ++i) {
         const float t = row16_sum(sum[i]);
-        if (n == i) {
-            const size_t at = (size_t)hkv * a.mass_ld + pos + i;
-            if (pos + i < a.n_past + a.M) a.mass_out[at] = a.mass_in[at] + t;
-        }
+        if (n == i) part[w][ch * 16 + i] = t;
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        const int t = tile * kKv8Tile + threadIdx.x;
+        const size_t at = (size_t)hkv * a.mass_ld + t;
+        float all = part[0][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < W; ++i) all += part[i][threadIdx.x];
+        if (t < a.n_past + a.M) a.mass_out[at] = a.mass_in[at] + all;
     }
 }
 // entries behind the slab's positions: carried over
@@ -1038,7 +1092,8 @@ hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_ou
 hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recent, const float* mass_in, int64_t ld_in, float* mass_out, int64_t ld_out, int32_t* kept,
                              hipStream_t st) {
 #define KV8_SELECT(N) hipLaunchKernelGGL(kv8_select_kernel<N>, dim3(Hkv), dim3(1024), 0, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept)
-    if (T <= 1024) KV8_SELECT(1);
+    if (T <= 512) hipLaunchKernelGGL(kv8_select_wave_kernel<8>, dim3(Hkv), dim3(64), 0, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept);
+    else if (T <= 1024) hipLaunchKernelGGL(kv8_select_wave_kernel<16>, dim3(Hkv), dim3(64), 0, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept);
     else if (T <= 4096) KV8_SELECT(4);
     else if (T <= 32768) KV8_SELECT(32);
     else KV8_SELECT(0);
@@ -1053,8 +1108,7 @@ hipError_t launch_kv8_move(const Kv8View& src, const Kv8View& dst, int n_keep, c
 template <typename F> static hipError_t lds_opt_in(F kernel, size_t bytes) {
     return bytes > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : hipSuccess;
 }
-template <int D> static hipError_t attn_tile(const Kv8Attn& a, hipStream_t st) {
-    constexpr int NC = D == 256 ? 1 : 2;
+template <int D, int NC> static hipError_t attn_tile(const Kv8Attn& a, hipStream_t st) {
     constexpr size_t lds = (size_t)2 * (4 * (D / 32) + 2 * (D / 16)) * 64 * 16;
     const int cols = a.M * (a.c.H / a.c.Hkv), blocks = (cols + 64 * NC - 1) / (64 * NC);
     const hipError_t e = lds_opt_in(kv8_attn_tile_kernel<D, NC>, lds);
@@ -1063,21 +1117,16 @@ template <int D> static hipError_t attn_tile(const Kv8Attn& a, hipStream_t st) {
     return hipGetLastError();
 }
 hipError_t launch_kv8_attn_tile(const Kv8Attn& a, hipStream_t st) {
-    KV8_BY_DIM(a.c.D, return attn_tile<kD>(a, st));
-    return hipErrorInvalidValue;
+    // 32 columns a wave halve the LDS reads of 16, once there are enough workgroups for every CU to hold two
+    const int64_t cols = (int64_t)a.M * (a.c.H / a.c.Hkv);
+    if (a.c.D == 256) return attn_tile<256, 1>(a, st);
+    if ((cols + 127) / 128 * a.c.Hkv >= 384) return a.c.D == 64 ? attn_tile<64, 2>(a, st) : attn_tile<128, 2>(a, st);
+    return a.c.D == 64 ? attn_tile<64, 1>(a, st) : attn_tile<128, 1>(a, st);
 }
 template <int D> static hipError_t mass_tile(const Kv8Attn& a, hipStream_t st) {
-    constexpr size_t lds = (size_t)4 * 2 * (D / 32) * 64 * 16 + 64 * 12;
     const int tiles = (a.n_past + a.M + kKv8Tile - 1) / kKv8Tile;
-    if (tiles * a.c.Hkv >= 2048) {
-        const hipError_t e = lds_opt_in(kv8_mass_tile_kernel<D, 4>, lds);
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((kv8_mass_tile_kernel<D, 4>), dim3((tiles + 3) / 4, a.c.Hkv), dim3(256), lds, st, a, kLog2e / sqrtf((float)D));
-    } else {
-        const hipError_t e = lds_opt_in(kv8_mass_tile_kernel<D, 1>, lds);
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((kv8_mass_tile_kernel<D, 1>), dim3(tiles, a.c.Hkv), dim3(256), lds, st, a, kLog2e / sqrtf((float)D));
-    }
+    constexpr int W = D == 256 ? 4 : 8;
+    hipLaunchKernelGGL((kv8_mass_tile_kernel<D, W>), dim3(tiles, a.c.Hkv), dim3(64 * W), 0, st, a, kLog2e / sqrtf((float)D));
     const int rest = a.mass_n - (a.n_past + a.M);
     if (rest > 0 && a.mass_in != a.mass_out) hipLaunchKernelGGL(kv8_mass_rest_kernel, dim3((rest + 255) / 256, a.c.Hkv), dim3(256), 0, st, a);
     return hipGetLastError();
