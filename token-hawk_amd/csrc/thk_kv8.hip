@@ -6,6 +6,9 @@
 
 namespace thk {
 
+__device__ __forceinline__ float as_f(unsigned v) { return __builtin_bit_cast(float, v); }
+__device__ __forceinline__ unsigned as_u(float v) { return __builtin_bit_cast(unsigned, v); }
+
 // ---------------------------------------------------------------- quantiser
 // A block's scale is f32(amax / 127), its codes rint(x * f32(127 / amax)).  fma with 1.5 * 2^23 rounds the exact product once, to the
 // nearest integer (ties to even): the code does not depend on a rounding of the product, and the low byte of the sum's bits is the code.
@@ -156,8 +159,15 @@ __device__ __forceinline__ unsigned mass_key(float x) {
     if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-// Exclusive prefix sum over 1024 threads; *total gets the sum.  sm: 16 words
-__device__ __forceinline__ unsigned block_scan_1024(unsigned v, unsigned* sm, unsigned* total) {
+// One workgroup per K/V head: the n_keep - n_sink - n_recent heaviest of the middle positions by radix selection, ties to the lowest position,
+// then the kept positions in ascending order.
+//   W waves; thread t takes positions 4 t .. 4 t + 3 of every 256 W.  With N > 0 (T <= 64 W N) their N keys stay in registers, else every pass
+//   reads the weights again, 64 a thread at a time.
+//   BITS a pass, histograms in LDS in R interleaved copies by lane (the weights' leading bits take few values, and copies in one bank
+//   would not help); thread t sums the buckets of one stretch, heaviest first.
+//   What stays is one ballot per 64 keys; the ballots' bit counts, summed up over waves, say where each thread's kept positions go.
+// What bounds it is one CU's instruction issue, so small sets take 4 waves instead of 16.
+template <int W> __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* sm, unsigned* total) {     // exclusive prefix sum over 64 W threads; sm: W words
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     unsigned s = v;
 #pragma unroll
@@ -167,180 +177,146 @@ __device__ __forceinline__ unsigned block_scan_1024(unsigned v, unsigned* sm, un
     __syncthreads();
     unsigned before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) { const unsigned t = sm[i]; if (i < w) before += t; all += t; }
+    for (int i = 0; i < W; ++i) { const unsigned t = sm[i]; if (i < w) before += t; all += t; }
     *total = all;
     return before + s - v;
 }
-// One workgroup per K/V head: the n_keep - n_sink - n_recent heaviest of the middle positions by radix selection (11, 11 and 10 bits of the
-// keys, histograms in LDS), ties to the lowest position, then the kept positions in ascending order.  Thread t has positions t + 1024 i; with
-// N > 0 (T <= 1024 N) their keys stay in registers, else every pass reads the weights again.  Which positions stay is written down as one
-// 64-bit ballot per 64 positions, whose bit counts, summed up, say where each wave's kept positions go; N = 0 does that 64 times 1024
-// positions at a time.
-static const int kKv8Hist = 4;
-template <int N>
-__global__ __launch_bounds__(1024) void kv8_select_kernel(int T, int n_keep, int n_sink, int n_recent, const float* __restrict__ mass_in, int64_t ld_in,
-                                                          float* __restrict__ mass_out, int64_t ld_out, int32_t* __restrict__ kept) {
-    constexpr int C = N > 0 ? N : 64;                                      // positions of a thread in one sweep
-    __shared__ unsigned hist[kKv8Hist][2048], sm[16], pick[2];            // copies by lane: the weights' leading bits take few values
-    __shared__ unsigned cnt[1024];                                         // [64 slices of 1024][16 waves]
+__device__ __forceinline__ float key_mass(unsigned k) { return as_f(k == 0 ? 0x7FC00000u : (k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }
+template <int W, int N, int BITS>
+__global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, int n_sink, int n_recent, const float* __restrict__ mass_in, int64_t ld_in,
+                                                            float* __restrict__ mass_out, int64_t ld_out, int32_t* __restrict__ kept) {
+    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+    constexpr int Q = (N > 0 ? N : 64) / 4, R = 4, B = 1 << BITS, PT = (B + 64 * W - 1) / (64 * W);     // groups of four a thread and sweep; copies; buckets; buckets a thread
+    __shared__ unsigned hist[B * R], sm[W], pick[3], cnt[Q * W];
     const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, lo = n_sink, hi = T - n_recent;
     const float* mass = mass_in + (size_t)h * ld_in;
-    unsigned need = (unsigned)(n_keep - n_sink - n_recent), prefix = 0;     // of the positions whose key starts with prefix, the `need` heaviest stay
-    float x[C];                                                            // the weights themselves: a key is three operations, a second read is not
-    auto key_at = [&](int t) { return mass_key(mass[t < T ? t : T - 1]); };
+    unsigned need = (unsigned)(n_keep - n_sink - n_recent), prefix = 0, same = 0;     // of the `same` positions whose key starts with prefix, the `need` heaviest stay
+    auto load4 = [&](int t, unsigned (&k)[4]) {                            // behind the end: some weight, not looked at
+        f4 v;
+        if (t + 3 < T) v = *reinterpret_cast<const f4u*>(mass + t);
+        else v = f4{mass[min(t, T - 1)], mass[min(t + 1, T - 1)], mass[min(t + 2, T - 1)], mass[T - 1]};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = mass_key(v[j]);
+    };
+    unsigned keys[N > 0 ? Q : 1][4];
     if (N > 0) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) x[i] = mass[min(i * 1024 + tid, T - 1)];
+        for (int q = 0; q < Q; ++q) load4((q * 64 * W + tid) * 4, keys[q]);
     }
-    int shift = 32;
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-        const int bits = pass < 2 ? 11 : 10, prev = shift;
-        shift -= bits;
-        const unsigned mask = (1u << bits) - 1;
-#pragma unroll
-        for (int i = 0; i < kKv8Hist; ++i) hist[i][tid] = hist[i][tid + 1024] = 0;
-        __syncthreads();
-        auto count = [&](int t, unsigned key) {
-            if (t >= lo && t < hi && (pass == 0 || (key >> prev) == prefix)) atomicAdd(&hist[lane % kKv8Hist][(key >> shift) & mask], 1u);    // integers: the order changes nothing
-        };
+    auto each = [&](int t0, auto f) {                                      // f(group, position, keys) over the sweep from t0
         if (N > 0) {
 #pragma unroll
-            for (int i = 0; i < C; ++i) count(i * 1024 + tid, mass_key(x[i]));
+            for (int q = 0; q < Q; ++q) f(q, (q * 64 * W + tid) * 4, keys[q]);
         } else {
-            for (int t = tid; t < T; t += 1024) count(t, key_at(t));
+#pragma unroll 1
+            for (int q = 0; q < Q; ++q) { unsigned k[4]; const int t = t0 + (q * 64 * W + tid) * 4; load4(t, k); f(q, t, k); }
         }
+    };
+    constexpr int SWEEP = Q * 256 * W;
+    int shift = 32;
+#pragma unroll 1
+    while (shift > 0) {
+        const int bits = shift < BITS ? shift : BITS, prev = shift;
+        const bool first = shift == 32;
+        shift -= bits;
+        const unsigned mask = (1u << bits) - 1;
+        for (int i = tid; i < B * R; i += 64 * W) hist[i] = 0;
         __syncthreads();
-        unsigned total;
-        const int top = (int)mask - 2 * tid;                               // thread i: buckets of digits top and top - 1, heaviest first
-        unsigned c0 = 0, c1 = 0;
-        if (top > 0) {
+        for (int t0 = 0; t0 < T; t0 += SWEEP)
+            each(t0, [&](int, int t, const unsigned (&k)[4]) {
 #pragma unroll
-            for (int i = 0; i < kKv8Hist; ++i) { c0 += hist[i][top]; c1 += hist[i][top - 1]; }
+                for (int j = 0; j < 4; ++j)
+                    if (t + j >= lo && t + j < hi && (first || (k[j] >> prev) == prefix)) atomicAdd(&hist[((k[j] >> shift) & mask) * R + lane % R], 1u);    // integers: the order changes nothing
+            });
+        __syncthreads();
+        unsigned c[PT], mine = 0, total;
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+            const int d = (int)mask - (tid * PT + i);
+            c[i] = 0;
+            if (d >= 0) { const uint4 v = *reinterpret_cast<const uint4*>(hist + d * R); c[i] = (v.x + v.y) + (v.z + v.w); }
+            mine += c[i];
         }
-        const unsigned above = block_scan_1024(c0 + c1, sm, &total);
-        if (above < need && need <= above + c0) { pick[0] = (unsigned)top; pick[1] = need - above; }
-        else if (above + c0 < need && need <= above + c0 + c1) { pick[0] = (unsigned)top - 1; pick[1] = need - above - c0; }
-        if (tid == 0 && need == 0) { pick[0] = mask; pick[1] = 0; }
+        unsigned above = block_scan<W>(mine, sm, &total);
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+            if (above < need && need <= above + c[i]) { pick[0] = mask - (unsigned)(tid * PT + i); pick[1] = need - above; pick[2] = c[i]; }
+            above += c[i];
+        }
+        if (tid == 0 && need == 0) { pick[0] = mask; pick[1] = pick[2] = 0; }
         __syncthreads();
-        prefix = (prefix << bits) | pick[0];
-        need = pick[1];
-        __syncthreads();
+        prefix = bits == 32 ? pick[0] : (prefix << bits) | pick[0];
+        need = pick[1]; same = pick[2];
     }
-    // of the positions equal to the threshold the first `need` stay: a sweep for their ranks, a sweep for the places of those that stay
-    unsigned eq_before = 0, kept_before = 0, all;
+    // stays: heavier than the threshold, or equal to it and among the first `need` of those
+    const bool all_ties = need == same;                                    // then nobody's rank matters
+    unsigned ties_before = 0, kept_before = 0, all;
 #pragma unroll 1
-    for (int t0 = 0; t0 < T; t0 += C * 1024) {
-        if (N == 0) {
-#pragma unroll 1
-            for (int i = 0; i < C; ++i) {
-                const int t = t0 + i * 1024 + tid;
-                const unsigned long long b = __ballot(t >= lo && t < hi && key_at(t) == prefix);
-                if (lane == 0) cnt[i * 16 + w] = (unsigned)__popcll(b);
-            }
-        } else {
+    for (int t0 = 0; t0 < T; t0 += SWEEP) {
+        const unsigned long long below = (1ull << lane) - 1;
+        auto place = [&](const bool (&f)[4], int (&at)[4]) {               // places of the set flags within the wave's 256 positions, and their number
+            unsigned long long b[4];
+            int n = 0, base = 0;
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                const int t = t0 + i * 1024 + tid;
-                const unsigned long long b = __ballot(t >= lo && t < hi && mass_key(x[i]) == prefix);
-                if (lane == 0) cnt[i * 16 + w] = (unsigned)__popcll(b);
-            }
-        }
-        __syncthreads();
-        const unsigned eq = block_scan_1024(tid < C * 16 ? cnt[tid] : 0u, sm, &all) + eq_before;
-        eq_before += all;
-        __syncthreads();
-        if (tid < C * 16) cnt[tid] = eq;
-        __syncthreads();
-        unsigned long long mine = 0;                                       // bit i: this thread's position i stays
-        auto decide = [&](int i, unsigned key) {
-            const int t = t0 + i * 1024 + tid;
-            const bool mid = t >= lo && t < hi, same = mid && key == prefix;
-            const unsigned long long b = __ballot(same);
-            const bool stay = t < T && (!mid || key > prefix || (same && cnt[i * 16 + w] + (unsigned)__popcll(b & ((1ull << lane) - 1)) < need));
-            mine |= (unsigned long long)stay << i;
+            for (int j = 0; j < 4; ++j) { b[j] = __ballot(f[j]); n += (int)__popcll(b[j]); base += (int)__popcll(b[j] & below); }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { at[j] = base; base += f[j]; }
+            return n;
         };
-        if (N == 0) {
-#pragma unroll 1
-            for (int i = 0; i < C; ++i) decide(i, key_at(t0 + i * 1024 + tid));
-        } else {
+        auto sum_up = [&](unsigned before) {                               // cnt -> what lies before each of its entries
+            __syncthreads();
+            static_assert(Q * W <= 64 * W, "one entry a thread");
+            const unsigned v = block_scan<W>(tid < Q * W ? cnt[tid] : 0u, sm, &all) + before;
+            if (tid < Q * W) cnt[tid] = v;
+            __syncthreads();
+        };
+        unsigned long long stay = 0;                                       // bit 4 q + j
+        if (!all_ties) {
+            each(t0, [&](int q, int t, const unsigned (&k)[4]) {
+                bool f[4]; int at[4];
 #pragma unroll
-            for (int i = 0; i < C; ++i) decide(i, mass_key(x[i]));
+                for (int j = 0; j < 4; ++j) f[j] = t + j >= lo && t + j < hi && k[j] == prefix;
+                const int n = place(f, at);
+                if (lane == 0) cnt[q * W + w] = (unsigned)n;
+            });
+            sum_up(ties_before);
+            ties_before += all;
         }
+        each(t0, [&](int q, int t, const unsigned (&k)[4]) {
+            bool mid[4], f[4]; int at[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { mid[j] = t + j >= lo && t + j < hi; f[j] = mid[j] && k[j] == prefix; }
+            if (!all_ties) place(f, at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool tie = f[j] && (all_ties ? need > 0 : cnt[q * W + w] + (unsigned)at[j] < need);
+                stay |= (unsigned long long)(t + j < T && (!mid[j] || k[j] > prefix || tie)) << (4 * q + j);
+            }
+        });
         __syncthreads();
-#pragma unroll 1
-        for (int i = 0; i < C; ++i) {
-            const unsigned long long b = __ballot(mine >> i & 1);
-            if (lane == 0) cnt[i * 16 + w] = (unsigned)__popcll(b);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) n += (int)__popcll(__ballot(stay >> (4 * q + j) & 1));
+            if (lane == 0) cnt[q * W + w] = (unsigned)n;
         }
-        __syncthreads();
-        const unsigned at0 = block_scan_1024(tid < C * 16 ? cnt[tid] : 0u, sm, &all) + kept_before;
+        sum_up(kept_before);
         kept_before += all;
+        each(t0, [&](int q, int t, const unsigned (&k)[4]) {
+            bool f[4]; int at[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = stay >> (4 * q + j) & 1;
+            place(f, at);
+            const unsigned base = cnt[q * W + w];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (f[j]) {
+                    kept[(size_t)h * n_keep + base + (unsigned)at[j]] = t + j;
+                    if (mass_out) mass_out[(size_t)h * ld_out + base + (unsigned)at[j]] = key_mass(k[j]);
+                }
+        });
         __syncthreads();
-        if (tid < C * 16) cnt[tid] = at0;
-        __syncthreads();
-        auto put = [&](int i, float v) {
-            const bool stay = mine >> i & 1;
-            const unsigned long long b = __ballot(stay);
-            if (stay) {
-                const unsigned at = cnt[i * 16 + w] + (unsigned)__popcll(b & ((1ull << lane) - 1));
-                kept[(size_t)h * n_keep + at] = t0 + i * 1024 + tid;
-                if (mass_out) mass_out[(size_t)h * ld_out + at] = v;
-            }
-        };
-        if (N == 0) {
-#pragma unroll 1
-            for (int i = 0; i < C; ++i) put(i, mass[min(t0 + i * 1024 + tid, T - 1)]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < C; ++i) put(i, x[i]);
-        }
-        __syncthreads();
-    }
-}
-// Few positions (T <= 64 N): one wave per head holds all keys, N a lane, and finds the threshold bit by bit with ballots - no LDS, no barrier.
-template <int N>
-__global__ __launch_bounds__(64) void kv8_select_wave_kernel(int T, int n_keep, int n_sink, int n_recent, const float* __restrict__ mass_in, int64_t ld_in,
-                                                             float* __restrict__ mass_out, int64_t ld_out, int32_t* __restrict__ kept) {
-    const int h = blockIdx.x, lane = threadIdx.x, lo = n_sink, hi = T - n_recent;
-    const float* mass = mass_in + (size_t)h * ld_in;
-    const int need = n_keep - n_sink - n_recent;
-    float x[N];
-    unsigned keys[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = mass[min(i * 64 + lane, T - 1)];
-    unsigned long long mid[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) { keys[i] = mass_key(x[i]); const int t = i * 64 + lane; mid[i] = __ballot(t >= lo && t < hi); }
-    unsigned thr = 0;                                                      // the largest value that `need` keys of the middle reach, two bits a turn
-#pragma unroll 1
-    for (int b = 30; b >= 0; b -= 2) {
-        int c[3] = {0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < 3; ++j) c[j] += (int)__popcll(__ballot(keys[i] >= (thr | (unsigned)(j + 1) << b)) & mid[i]);
-        thr |= (c[2] >= need ? 3u : c[1] >= need ? 2u : c[0] >= need ? 1u : 0u) << b;
-    }
-    int above = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) above += (int)__popcll(__ballot(keys[i] > thr) & mid[i]);
-    int ties = need - above, at = 0;                                       // of those equal to it the first `ties` stay
-    const unsigned long long below = (1ull << lane) - 1;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int t = i * 64 + lane;
-        const unsigned long long same = __ballot(keys[i] == thr) & mid[i];
-        const bool in = mid[i] >> lane & 1;
-        const bool stay = t < T && (!in || (need > 0 && (keys[i] > thr || (keys[i] == thr && (int)__popcll(same & below) < ties))));
-        ties -= (int)__popcll(same);
-        const unsigned long long s = __ballot(stay);
-        if (stay) {
-            const size_t to = (size_t)(at + (int)__popcll(s & below));
-            kept[(size_t)h * n_keep + to] = t;
-            if (mass_out) mass_out[(size_t)h * ld_out + to] = x[i];
-        }
-        at += (int)__popcll(s);
     }
 }
 // One workgroup per destination block, head and K | V: gathers the 16 kept rows as values and quantises them anew.  Sixteen rows that were
@@ -428,8 +404,6 @@ __device__ __forceinline__ U2 pair32(unsigned v) {
     const auto r = __builtin_amdgcn_permlane32_swap(v, w, false, false);
     return {r[0], r[1]};
 }
-__device__ __forceinline__ float as_f(unsigned v) { return __builtin_bit_cast(float, v); }
-__device__ __forceinline__ unsigned as_u(float v) { return __builtin_bit_cast(unsigned, v); }
 // over the four lanes of a column
 __device__ __forceinline__ float chunks_max(float v) {
     U2 r = pair16(as_u(v));
@@ -1091,12 +1065,11 @@ hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_ou
 }
 hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recent, const float* mass_in, int64_t ld_in, float* mass_out, int64_t ld_out, int32_t* kept,
                              hipStream_t st) {
-#define KV8_SELECT(N) hipLaunchKernelGGL(kv8_select_kernel<N>, dim3(Hkv), dim3(1024), 0, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept)
-    if (T <= 512) hipLaunchKernelGGL(kv8_select_wave_kernel<8>, dim3(Hkv), dim3(64), 0, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept);
-    else if (T <= 1024) hipLaunchKernelGGL(kv8_select_wave_kernel<16>, dim3(Hkv), dim3(64), 0, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept);
-    else if (T <= 4096) KV8_SELECT(4);
-    else if (T <= 32768) KV8_SELECT(32);
-    else KV8_SELECT(0);
+#define KV8_SELECT(W, N, BITS) hipLaunchKernelGGL((kv8_select_kernel<W, N, BITS>), dim3(Hkv), dim3(64 * W), 0, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept)
+    if (T <= 1024) KV8_SELECT(4, 4, 8);
+    else if (T <= 4096) KV8_SELECT(16, 4, 11);
+    else if (T <= 32768) KV8_SELECT(16, 32, 11);
+    else KV8_SELECT(16, 0, 11);
 #undef KV8_SELECT
     return hipGetLastError();
 }
