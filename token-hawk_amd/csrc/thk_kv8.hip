@@ -41,6 +41,13 @@ template <int D, bool V> __device__ __forceinline__ int el_row(int i) { return V
 template <int D, bool V> __device__ __forceinline__ int el_dim(int i) { return V ? (int)(threadIdx.x % D) : (int)(threadIdx.x & 15) * (D / 16) + i; }
 template <int D, bool V> __device__ __forceinline__ int code_at() { return V ? (int)(threadIdx.x % D) * 16 + (int)(threadIdx.x / D) * (D / 16) : (int)threadIdx.x * (D / 16); }
 
+template <int D> __device__ __forceinline__ void get_codes(const int8_t* p, int (&q)[D / 16]) {
+    int w[D / 64];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) w[i] = reinterpret_cast<const int*>(p)[i];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) q[i] = (int)(int8_t)(w[i / 4] >> (8 * (i % 4)));
+}
 template <int D> __device__ __forceinline__ void put_codes(int8_t* p, const unsigned (&q)[D / 16]) {
     unsigned* w = reinterpret_cast<unsigned*>(p);
 #pragma unroll
@@ -80,13 +87,13 @@ __device__ void append_block(const Kv8View& c, int h, int b, const float* x, int
         const int2 t = *at;
         const float old = *scale;
         float xn[D / 16], xt[D / 16];
-        int8_t xc[D / 16];
+        int xc[D / 16];
+        get_codes<D>(codes, xc);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
             const int r = el_row<D, V>(i), d = el_dim<D, V>(i);
             xn[i] = src[(size_t)min(max(r, r0), r1 - 1) * ld + d];
             xt[i] = tail[r * D + d];
-            xc[i] = codes[i];
         }
         const int held = t.x == b ? t.y : 0;
 #pragma unroll
@@ -131,8 +138,10 @@ __device__ __forceinline__ void read_body(const Kv8View& c, int64_t pos, int64_t
     const int8_t* codes = (V ? c.v : c.k) + hb * (kKv8Block * D) + code_at<D, V>();
     const float s = (V ? c.vs : c.ks)[hb];
     float xs[D / 16];
+    int q[D / 16];
+    get_codes<D>(codes, q);
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) xs[i] = (float)codes[i] * s;
+    for (int i = 0; i < D / 16; ++i) xs[i] = (float)q[i] * s;
     const int64_t p0 = (int64_t)b * kKv8Block - pos, ld = (int64_t)c.Hkv * D;
     float* to = out + p0 * ld + (int64_t)h * D + el_dim<D, V>(0);          // row r of the block: to + r ld
     if (V) {
@@ -153,17 +162,19 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8View c, int64_t pos, i
 }
 
 // ---------------------------------------------------------------- eviction
-// Weights as unsigned keys, heaviest first: order-preserving, -0 = +0, NaN (the weight of a row nobody could attend) below everything.
+// Weights as unsigned keys, heaviest first: order-preserving, -0 = +0, NaN (the weight of a row nobody could attend) below everything but the
+// 0 of a position that does not exist; the positions that stay whatever their weight have the largest.
+static const unsigned kKeyStays = 0xFFFFFFFFu;
 __device__ __forceinline__ unsigned mass_key(float x) {
-    const unsigned b = __builtin_bit_cast(unsigned, x + 0.f);
-    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
+    const unsigned b = as_u(x + 0.f);
+    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 1u;
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-// One workgroup per K/V head: the n_keep - n_sink - n_recent heaviest of the middle positions by radix selection, ties to the lowest position,
-// then the kept positions in ascending order.
-//   W waves; thread t takes positions 4 t .. 4 t + 3 of every 256 W.  With N > 0 (T <= 64 W N) their N keys stay in registers, else every pass
-//   reads the weights again, 64 a thread at a time.
-//   BITS a pass, histograms in LDS in R interleaved copies by lane (the weights' leading bits take few values, and copies in one bank
+__device__ __forceinline__ float key_mass(unsigned k) { return as_f(k == 1u ? 0x7FC00000u : (k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }
+// One workgroup per K/V head: the n_keep largest keys by radix selection, ties to the lowest position, then the kept positions in ascending order.
+//   W waves; thread t takes positions 4 t .. 4 t + 3 of every 256 W.  With N > 0 (T <= 64 W N) their N keys stay in LDS, else every pass reads
+//   the weights again, 64 a thread at a time.  (Registers would hold them too, but loops over them have to be unrolled, and then spill.)
+//   BITS a pass, histograms in LDS in two interleaved copies by lane (the weights' leading bits take few values, and copies in one bank
 //   would not help); thread t sums the buckets of one stretch, heaviest first.
 //   What stays is one ballot per 64 keys; the ballots' bit counts, summed up over waves, say where each thread's kept positions go.
 // What bounds it is one CU's instruction issue, so small sets take 4 waves instead of 16.
@@ -181,35 +192,40 @@ template <int W> __device__ __forceinline__ unsigned block_scan(unsigned v, unsi
     *total = all;
     return before + s - v;
 }
-__device__ __forceinline__ float key_mass(unsigned k) { return as_f(k == 0 ? 0x7FC00000u : (k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }
 template <int W, int N, int BITS>
 __global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, int n_sink, int n_recent, const float* __restrict__ mass_in, int64_t ld_in,
                                                             float* __restrict__ mass_out, int64_t ld_out, int32_t* __restrict__ kept) {
     typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
-    constexpr int Q = (N > 0 ? N : 64) / 4, R = 4, B = 1 << BITS, PT = (B + 64 * W - 1) / (64 * W);     // groups of four a thread and sweep; copies; buckets; buckets a thread
+    constexpr int Q = (N > 0 ? N : 64) / 4, R = 2, B = 1 << BITS, PT = (B + 64 * W - 1) / (64 * W);     // groups of four a thread and sweep; copies; buckets; buckets a thread
     __shared__ unsigned hist[B * R], sm[W], pick[3], cnt[Q * W];
+    extern __shared__ __align__(16) char smem[];
+    uint4* keys = reinterpret_cast<uint4*>(smem);                          // [Q][64 W]
     const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, lo = n_sink, hi = T - n_recent;
     const float* mass = mass_in + (size_t)h * ld_in;
-    unsigned need = (unsigned)(n_keep - n_sink - n_recent), prefix = 0, same = 0;     // of the `same` positions whose key starts with prefix, the `need` heaviest stay
-    auto load4 = [&](int t, unsigned (&k)[4]) {                            // behind the end: some weight, not looked at
+    unsigned need = (unsigned)n_keep, prefix = 0, same = 0;                // of the `same` positions whose key starts with prefix, the `need` heaviest stay
+    auto load4 = [&](int t, unsigned (&k)[4]) {
         f4 v;
         if (t + 3 < T) v = *reinterpret_cast<const f4u*>(mass + t);
         else v = f4{mass[min(t, T - 1)], mass[min(t + 1, T - 1)], mass[min(t + 2, T - 1)], mass[T - 1]};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) k[j] = mass_key(v[j]);
+        for (int j = 0; j < 4; ++j) k[j] = t + j >= T ? 0u : t + j < lo || t + j >= hi ? kKeyStays : mass_key(v[j]);
     };
-    unsigned keys[N > 0 ? Q : 1][4];
-    if (N > 0) {
-#pragma unroll
-        for (int q = 0; q < Q; ++q) load4((q * 64 * W + tid) * 4, keys[q]);
+    if (N > 0) {                                                           // read by the thread that writes them
+#pragma unroll 4
+        for (int q = 0; q < Q; ++q) {
+            unsigned k[4];
+            load4((q * 64 * W + tid) * 4, k);
+            keys[q * 64 * W + tid] = uint4{k[0], k[1], k[2], k[3]};
+        }
     }
     auto each = [&](int t0, auto f) {                                      // f(group, position, keys) over the sweep from t0
-        if (N > 0) {
-#pragma unroll
-            for (int q = 0; q < Q; ++q) f(q, (q * 64 * W + tid) * 4, keys[q]);
-        } else {
-#pragma unroll 1
-            for (int q = 0; q < Q; ++q) { unsigned k[4]; const int t = t0 + (q * 64 * W + tid) * 4; load4(t, k); f(q, t, k); }
+#pragma unroll 4
+        for (int q = 0; q < Q; ++q) {
+            unsigned k[4];
+            const int t = t0 + (q * 64 * W + tid) * 4;
+            if (N > 0) { const uint4 v = keys[q * 64 * W + tid]; k[0] = v.x; k[1] = v.y; k[2] = v.z; k[3] = v.w; }
+            else load4(t, k);
+            f(q, t, k);
         }
     };
     constexpr int SWEEP = Q * 256 * W;
@@ -223,10 +239,10 @@ __global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, i
         for (int i = tid; i < B * R; i += 64 * W) hist[i] = 0;
         __syncthreads();
         for (int t0 = 0; t0 < T; t0 += SWEEP)
-            each(t0, [&](int, int t, const unsigned (&k)[4]) {
+            each(t0, [&](int, int, const unsigned (&k)[4]) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (t + j >= lo && t + j < hi && (first || (k[j] >> prev) == prefix)) atomicAdd(&hist[((k[j] >> shift) & mask) * R + lane % R], 1u);    // integers: the order changes nothing
+                    if (first || (k[j] >> prev) == prefix) atomicAdd(&hist[((k[j] >> shift) & mask) * R + lane % R], 1u);    // integers: the order changes nothing
             });
         __syncthreads();
         unsigned c[PT], mine = 0, total;
@@ -234,7 +250,7 @@ __global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, i
         for (int i = 0; i < PT; ++i) {
             const int d = (int)mask - (tid * PT + i);
             c[i] = 0;
-            if (d >= 0) { const uint4 v = *reinterpret_cast<const uint4*>(hist + d * R); c[i] = (v.x + v.y) + (v.z + v.w); }
+            if (d >= 0) { const uint2 v = *reinterpret_cast<const uint2*>(hist + d * R); c[i] = v.x + v.y; }
             mine += c[i];
         }
         unsigned above = block_scan<W>(mine, sm, &total);
@@ -243,7 +259,6 @@ __global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, i
             if (above < need && need <= above + c[i]) { pick[0] = mask - (unsigned)(tid * PT + i); pick[1] = need - above; pick[2] = c[i]; }
             above += c[i];
         }
-        if (tid == 0 && need == 0) { pick[0] = mask; pick[1] = pick[2] = 0; }
         __syncthreads();
         prefix = bits == 32 ? pick[0] : (prefix << bits) | pick[0];
         need = pick[1]; same = pick[2];
@@ -270,50 +285,51 @@ __global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, i
             if (tid < Q * W) cnt[tid] = v;
             __syncthreads();
         };
-        unsigned long long stay = 0;                                       // bit 4 q + j
+        unsigned long long ties = 0;                                       // bit 4 q + j: equal to the threshold and among the first
         if (!all_ties) {
-            each(t0, [&](int q, int t, const unsigned (&k)[4]) {
+            each(t0, [&](int q, int, const unsigned (&k)[4]) {
                 bool f[4]; int at[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) f[j] = t + j >= lo && t + j < hi && k[j] == prefix;
+                for (int j = 0; j < 4; ++j) f[j] = k[j] == prefix;
                 const int n = place(f, at);
                 if (lane == 0) cnt[q * W + w] = (unsigned)n;
             });
             sum_up(ties_before);
             ties_before += all;
+            each(t0, [&](int q, int, const unsigned (&k)[4]) {
+                bool f[4]; int at[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[j] = k[j] == prefix;
+                place(f, at);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ties |= (unsigned long long)(f[j] && cnt[q * W + w] + (unsigned)at[j] < need) << (4 * q + j);
+            });
+            __syncthreads();
         }
-        each(t0, [&](int q, int t, const unsigned (&k)[4]) {
-            bool mid[4], f[4]; int at[4];
+        auto stays = [&](int q, const unsigned (&k)[4], bool (&f)[4]) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { mid[j] = t + j >= lo && t + j < hi; f[j] = mid[j] && k[j] == prefix; }
-            if (!all_ties) place(f, at);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool tie = f[j] && (all_ties ? need > 0 : cnt[q * W + w] + (unsigned)at[j] < need);
-                stay |= (unsigned long long)(t + j < T && (!mid[j] || k[j] > prefix || tie)) << (4 * q + j);
-            }
-        });
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
+            for (int j = 0; j < 4; ++j) f[j] = all_ties ? k[j] >= prefix : k[j] > prefix || (ties >> (4 * q + j) & 1);
+        };
+        each(t0, [&](int q, int, const unsigned (&k)[4]) {
+            bool f[4];
+            stays(q, k, f);
             int n = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) n += (int)__popcll(__ballot(stay >> (4 * q + j) & 1));
+            for (int j = 0; j < 4; ++j) n += (int)__popcll(__ballot(f[j]));
             if (lane == 0) cnt[q * W + w] = (unsigned)n;
-        }
+        });
         sum_up(kept_before);
         kept_before += all;
         each(t0, [&](int q, int t, const unsigned (&k)[4]) {
             bool f[4]; int at[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = stay >> (4 * q + j) & 1;
+            stays(q, k, f);
             place(f, at);
             const unsigned base = cnt[q * W + w];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (f[j]) {
                     kept[(size_t)h * n_keep + base + (unsigned)at[j]] = t + j;
-                    if (mass_out) mass_out[(size_t)h * ld_out + base + (unsigned)at[j]] = key_mass(k[j]);
+                    if (mass_out) mass_out[(size_t)h * ld_out + base + (unsigned)at[j]] = k[j] == kKeyStays ? mass[t + j] : key_mass(k[j]);
                 }
         });
         __syncthreads();
@@ -332,12 +348,20 @@ __device__ __forceinline__ void move_body(const Kv8View& s, const Kv8View& d, in
     const size_t hb = (size_t)h * d.n_blk + b;
     float xs[D / 16], sc_[D / 16];
     unsigned q[D / 16], m = 0;
-    int8_t code[D / 16];
+    int code[D / 16];
+    if (V) {
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {                                     // rows behind the last kept one read position 0: all loads at once
-        const int p = max(src[el_row<D, V>(i)], 0), dim = el_dim<D, V>(i);
-        code[i] = V ? from[((size_t)(p >> 4) * D + dim) * 16 + (p & 15)] : from[(size_t)p * D + dim];
-        sc_[i] = sc[p >> 4];
+        for (int i = 0; i < D / 16; ++i) {                                 // rows behind the last kept one read position 0: all loads at once
+            const int p = max(src[el_row<D, V>(i)], 0);
+            code[i] = from[((size_t)(p >> 4) * D + el_dim<D, V>(0)) * 16 + (p & 15)];
+            sc_[i] = sc[p >> 4];
+        }
+    } else {
+        const int p = max(src[el_row<D, V>(0)], 0);
+        get_codes<D>(from + (size_t)p * D + el_dim<D, V>(0), code);
+        const float s0 = sc[p >> 4];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) sc_[i] = s0;
     }
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
@@ -1044,6 +1068,10 @@ __global__ __launch_bounds__(256) void kv8_mass_rest_kernel(Kv8Attn a) {
 }
 
 // ---------------------------------------------------------------- launchers
+template <typename F> static hipError_t lds_opt_in(F kernel, size_t bytes) {
+    return bytes > 32768 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : hipSuccess;
+}
+
 #define KV8_BY_DIM(D, EXPR)                                   \
     switch (D) {                                              \
         case 64: { constexpr int kD = 64; EXPR; break; }      \
@@ -1065,7 +1093,14 @@ hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_ou
 }
 hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recent, const float* mass_in, int64_t ld_in, float* mass_out, int64_t ld_out, int32_t* kept,
                              hipStream_t st) {
-#define KV8_SELECT(W, N, BITS) hipLaunchKernelGGL((kv8_select_kernel<W, N, BITS>), dim3(Hkv), dim3(64 * W), 0, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept)
+#define KV8_SELECT(W, N, BITS)                                                                                                                       \
+    do {                                                                                                                                           \
+        const size_t lds = (size_t)N * 64 * W * 4;                                                                                                 \
+        const hipError_t e = lds_opt_in(kv8_select_kernel<W, N, BITS>, lds);                                                                       \
+        if (e != hipSuccess) return e;                                                                                                             \
+        hipLaunchKernelGGL((kv8_select_kernel<W, N, BITS>), dim3(Hkv), dim3(64 * W), lds, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, \
+                           ld_out, kept);                                                                                                          \
+    } while (0)
     if (T <= 1024) KV8_SELECT(4, 4, 8);
     else if (T <= 4096) KV8_SELECT(16, 4, 11);
     else if (T <= 32768) KV8_SELECT(16, 32, 11);
@@ -1077,9 +1112,6 @@ hipError_t launch_kv8_move(const Kv8View& src, const Kv8View& dst, int n_keep, c
     const dim3 grid((unsigned)((n_keep + kKv8Block - 1) / kKv8Block), src.Hkv, 2);
     KV8_BY_DIM(src.D, hipLaunchKernelGGL(kv8_move_kernel<kD>, grid, dim3(256), 0, st, src, dst, n_keep, kept));
     return hipGetLastError();
-}
-template <typename F> static hipError_t lds_opt_in(F kernel, size_t bytes) {
-    return bytes > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : hipSuccess;
 }
 template <int D, int NC> static hipError_t attn_tile(const Kv8Attn& a, hipStream_t st) {
     constexpr size_t lds = (size_t)2 * (4 * (D / 32) + 2 * (D / 16)) * 64 * 16;
