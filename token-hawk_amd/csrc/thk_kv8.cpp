@@ -58,7 +58,7 @@ extern "C" int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_
     const size_t codes = (size_t)H_kv * v.n_blk * kKv8Block * D, scales = up256((size_t)H_kv * v.n_blk * 4), tail = (size_t)2 * H_kv * kKv8Block * D * 4;
     const size_t at = up256((size_t)2 * H_kv * sizeof(int2)), ml = (size_t)kKv8RowSlab * H * sizeof(float2);
     const size_t part = (size_t)kKv8SplitRows * (D * 4 + sizeof(float2)), scores_bytes = (size_t)H * v.n_blk * kKv8Block * 4;
-    kv->mem_bytes = 2 * codes + 2 * scales + tail + at + ml + part + kKv8Counters * 4 + scores_bytes;
+    kv->mem_bytes = 2 * codes + 2 * scales + tail + at + ml + part + kKv8Groups * 4 + scores_bytes;
     hipError_t e = hipMalloc(&kv->mem, kv->mem_bytes);
     if (e != hipSuccess) {
         (void)hipGetLastError();
@@ -76,7 +76,7 @@ extern "C" int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_
     kv->ml = (float2*)p; p += ml;
     kv->part_o = (float*)p; p += (size_t)kKv8SplitRows * D * 4;
     kv->part_ml = (float2*)p; p += (size_t)kKv8SplitRows * sizeof(float2);
-    kv->counters = (unsigned*)p; p += kKv8Counters * 4;
+    kv->counters = (unsigned*)p; p += kKv8Groups * 4;
     kv->scores = (float*)p;
     e = hipMemsetAsync(kv->mem, 0, kv->mem_bytes, ctx->stream);
     if (e == hipSuccess) e = hipMemsetAsync(v.tail_at, 0xFF, (size_t)2 * H_kv * sizeof(int2), ctx->stream);     // no block is open
@@ -142,20 +142,22 @@ static int kv8_attention(thk_kv8* kv, const char* what, const float* q, int64_t 
         if (mass_out) { a.ml = kv->ml; a.mass_in = mass_in; a.mass_out = mass_out; a.mass_ld = kv->n_ctx; a.mass_n = (int)(n_past + M); }
         bool scored = false;
         const int64_t G = a.c.H / a.c.Hkv, cols = a.M * G, cg = (cols + 15) / 16, groups = cg * a.c.Hkv;      // workgroups without a split
-        auto env = [](const char* n, int64_t d) { const char* e = getenv(n); return e ? (int64_t)atoll(e) : d; };
-        if (cols <= env("KV8_COLS", 64)) {
+        // Few columns: split over the positions, a tile of 64 a wave in turn; many: whole rows, tiles shared by a workgroup.  At 512 positions x 1024
+        // groups 29 | 18 us, at 8192 x 512 groups 100 | 190, x 1024 groups 185 | 196 (split | rows): the border is at 512 groups.
+        if (groups <= kKv8Groups) {
             Kv8Split sp{};
-            sp.waves = a.c.D == 256 ? 4 : (int)env("KV8_W", 8);
-            const int64_t T = a.n_past + a.M, tiles = (T + kKv8Tile - 1) / kKv8Tile, most = (tiles + sp.waves - 1) / sp.waves;
-            int64_t n = env("KV8_WG", sp.waves == 8 ? 256 : 512) / groups;
-            if (n > most) n = most;
-            if (n > 64) n = 64;
-            if (n > kKv8SplitRows / ((int64_t)a.M * a.c.H)) n = kKv8SplitRows / ((int64_t)a.M * a.c.H);
+            const int64_t T = a.n_past + a.M, tiles = (T + kKv8Tile - 1) / kKv8Tile, waves = kv8_split_waves(a.c.D);
+            // one workgroup on every CU, at least a tile for every wave
+            const int64_t n = std::min({256 / groups, (tiles + waves - 1) / waves, (int64_t)64, kKv8SplitRows / ((int64_t)a.M * a.c.H)});
             sp.n = n < 1 ? 1 : (int)n; sp.part_o = kv->part_o; sp.part_ml = kv->part_ml;
-            sp.stream = cg == 1 && 2 * T * a.c.Hkv * a.c.D >= env("KV8_NTB", 64 << 20);
-            if (mass_out && a.M == 1 && G <= 16) { scored = true; sp.scores = kv->scores; sp.scores_ld = (int64_t)a.c.n_blk * kKv8Block; }
-            const bool join = sp.n * std::min<int64_t>(cols, 16) <= env("KV8_JOIN", 64) && (!scored || T * G <= env("KV8_JOINT", 8192));
-            if (groups <= kKv8Counters && join && (sp.n > 1 || scored)) sp.counters = kv->counters;
+            sp.stream = cg == 1 && 2 * T * a.c.Hkv * a.c.D >= (64 << 20);  // twice what the L2s hold: 112 -> 100 us at 65535 x 32 heads; at 2047 x 40 heads 10.4 -> 11.1
+            // Joined inside the launch where the last workgroup has little to do: 4096 positions, 32 heads on 8, 10.4 -> 9.7 us, at 8192 10.8 -> 11.3; and
+            // the weights counted there, too: 2048 positions 17.4 -> 13.2 us, 8192 19.6 -> 23.3.
+            const bool inside = sp.n * std::min<int64_t>(cols, 16) <= 64, count = mass_out && a.M == 1 && G <= 16;
+            const bool count_inside = inside && T <= 4096;
+            scored = count && (count_inside || sp.n > 1);
+            if (scored) { sp.scores = kv->scores; sp.scores_ld = (int64_t)a.c.n_blk * kKv8Block; }
+            if (scored ? count_inside : inside && sp.n > 1) sp.counters = kv->counters;
             HIPCHK(ctx, launch_kv8_attn_split(a, sp, ctx->stream));
         } else HIPCHK(ctx, launch_kv8_attn_tile(a, ctx->stream));
         if (mass_out && !scored) HIPCHK(ctx, launch_kv8_attn_mass(a, ctx->stream));

@@ -462,28 +462,43 @@ __device__ __forceinline__ void load_q(const float* q, bool valid, f4 (&x)[D / 1
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) x[i] = valid ? reinterpret_cast<const f4*>(q)[(i / 4) * 16 + i % 4] : f4{0.f, 0.f, 0.f, 0.f};
 }
-template <int D>
-__device__ __forceinline__ float q_digits(const f4 (&x)[D / 16], i4 (&qd)[3][D / 64]) {
+// digits of 4 N numbers of a lane as fixed point relative to the largest of their column, as put(word, d2, d1, d0); returns its step
+template <int N, typename Max, typename Put>
+__device__ __forceinline__ float digits_of(const f4 (&x)[N], Max column_max, Put put) {
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) { const unsigned a = abs_bits(x[i][j]); m = a > m ? a : m; }
-    m = chunks_max_bits(m);
+    m = column_max(m);
     const float amax = as_f(m);
     const bool some = amax >= 0x1p-100f;                                   // also false for NaN
     const float inv = some && m < 0x7F800000u ? 8355000.f / amax : 0.f;    // below 127 (2^16 + 2^8 + 1), the largest sum of three balanced digits, by more than the roundings
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
+    for (int i = 0; i < N; ++i) {
         unsigned e[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[j] = (unsigned)((int)rintf(x[i][j] * inv) + 0x808080);
         int d2, d1, d0;
         pack_digits<true>(e[0], e[1], e[2], e[3], d2, d1, d0);
-        qd[2][i / 4][i % 4] = d2; qd[1][i / 4][i % 4] = d1; qd[0][i / 4][i % 4] = d0;
+        put(i, d2, d1, d0);
     }
     if (m >= 0x7F800000u) return as_f(0x7FC00000u);                        // a query that is not finite: every score is NaN
     return some ? amax / 8355000.f : 0.f;
+}
+template <int D>
+__device__ __forceinline__ float q_digits(const f4 (&x)[D / 16], i4 (&qd)[3][D / 64]) {
+    return digits_of<D / 16>(x, chunks_max_bits, [&](int i, int d2, int d1, int d0) { qd[2][i / 4][i % 4] = d2; qd[1][i / 4][i % 4] = d1; qd[0][i / 4][i % 4] = d0; });
+}
+template <int CTRL> __device__ __forceinline__ unsigned dpp_max(unsigned v) {
+    const unsigned u = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+    return u > v ? u : v;
+}
+template <int L> __device__ __forceinline__ unsigned row_max_bits(unsigned v) {      // over aligned groups of L = 16, 32 or 64 lanes
+    v = dpp_max<0x140>(dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(v))));
+    if (L >= 32) { const U2 r = pair16(v); v = r.a > r.b ? r.a : r.b; }
+    if (L >= 64) { const U2 r = pair32(v); v = r.a > r.b ? r.a : r.b; }
+    return v;
 }
 // What one workgroup leaves for another inside a launch is written and read past the XCDs' own L2s (agent scope).
 __device__ __forceinline__ void put2(float* p, float x, float y) { st_agent_u64(reinterpret_cast<unsigned long long*>(p), (unsigned long long)as_u(y) << 32 | as_u(x)); }
@@ -497,7 +512,7 @@ template <bool NT> __device__ __forceinline__ i4 load16(const void* p) {
 template <int D, int W, bool NT>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_attn_split_kernel(Kv8Attn a, Kv8Split sp, float scale) {
     constexpr int KC = D / 64, NG = D / 16;
-    __shared__ float so[W][16][D + 4], sml[W][16][2];
+    __shared__ float so[W][16][D + 4], sml[W][16][2], fin[2][16];     // fin: maximum and 1 / sum of the columns, once they are final
     __shared__ int last;
     const Kv8View& c = a.c;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, ch = lane >> 4;
@@ -509,8 +524,18 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_attn_split_kerne
     const size_t orow = valid ? (size_t)row * c.H + hkv * G + (col - row * G) : 0;
     auto out_row = [&](int cc) { const int i = one ? 0 : cc / G; return (size_t)i * c.H + hkv * G + (cc - i * G); };
 
-    f4 qx[D / 16];
-    load_q<D>(a.q + orow * D + ch * 16, valid, qx);
+    // q's digits, by all threads together (a wave alone would spend as long on one column as on sixteen): a thread has four dimensions
+    constexpr int QL = D / 4 + 4;                                    // words of a column in LDS, padded against bank conflicts
+    __shared__ unsigned sq[3][16][QL];
+    __shared__ float sqf[16];
+    const int nv = min(cols - (int)blockIdx.z * 16, 16);
+    constexpr int QN = (16 * (D / 4) + 64 * W - 1) / (64 * W);
+    f4 qx[QN];
+#pragma unroll
+    for (int k = 0; k < QN; ++k) {
+        const int j = threadIdx.x + k * 64 * W;
+        if (j < nv * (D / 4)) qx[k] = reinterpret_cast<const f4*>(a.q + out_row(blockIdx.z * 16 + j / (D / 4)) * D)[j % (D / 4)];
+    }
     const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + 16 * (n >> 2) + (n & 3)) * D + ch * 16;
     const int8_t* vb = c.v + (((size_t)hkv * c.n_blk + ch) * D + n) * 16;
     const float *ksb = c.ks + (size_t)hkv * c.n_blk + ch, *vsb = c.vs + (size_t)hkv * c.n_blk + ch;
@@ -532,8 +557,22 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_attn_split_kerne
     };
     int t = split * per + w;
     if (t < t1) { load_k(t); load_v(t); }
-    i4 qd[3][KC];
-    const float qf = q_digits<D>(qx, qd) * scale;
+#pragma unroll
+    for (int k = 0; k < QN; ++k) {
+        const int j = threadIdx.x + k * 64 * W, cn = j / (D / 4);
+        if (j < nv * (D / 4)) {
+            const f4 x[1] = {qx[k]};
+            const float step = digits_of<1>(x, row_max_bits<D / 4>, [&](int, int d2, int d1, int d0) { sq[2][cn][j % (D / 4)] = d2; sq[1][cn][j % (D / 4)] = d1; sq[0][cn][j % (D / 4)] = d0; });
+            if (j % (D / 4) == 0) sqf[cn] = step * scale;
+        }
+    }
+    __syncthreads();
+    i4 qd[3][KC];                                                    // columns behind the last: whatever is there, times 0
+#pragma unroll
+    for (int d = 0; d < 3; ++d)
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) qd[d][kc] = *reinterpret_cast<const i4*>(&sq[d][n][16 * kc + 4 * ch]);
+    const float qf = valid ? sqf[n] : 0.f;
     float m = -INFINITY, l = 0.f;
     f4 o[NG];
 #pragma unroll
@@ -625,7 +664,6 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_attn_split_kerne
         if (ch == 0) { sml[w][n][0] = m; sml[w][n][1] = l; }
     }
     __syncthreads();
-    const int nv = min(cols - (int)blockIdx.z * 16, 16);
     for (int j = threadIdx.x; j < nv * (D / 4); j += 64 * W) {
         const int cn = j / (D / 4), d = (j % (D / 4)) * 4, cc = blockIdx.z * 16 + cn;
         const size_t r = out_row(cc);
@@ -654,99 +692,140 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_attn_split_kerne
             put2(po, sum[0], sum[1]); put2(po + 2, sum[2], sum[3]);
         }
         if (d == 0) {
-            if (sp.n > 1 || sp.counters) put2(reinterpret_cast<float*>(sp.part_ml + r * sp.n + split), mm, ll);
-            if (sp.n == 1 && a.ml) a.ml[r] = float2{mm, ll};
+            if (sp.n == 1) {
+                fin[0][cn] = mm; fin[1][cn] = 1.f / ll;
+                if (a.ml) a.ml[r] = float2{mm, ll};
+            } else put2(reinterpret_cast<float*>(sp.part_ml + r * sp.n + split), mm, ll);
         }
     }
     if (!sp.counters) return;
     // The workgroup that finishes last for its columns joins the splits (in their order, whoever comes last) and counts the weights.
-    unsigned* counter = sp.counters + blockIdx.z * gridDim.y + hkv;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                 // this thread's parts and scores are where the others can see them
     __syncthreads();
-    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)sp.n - 1;
-    __syncthreads();
-    if (!last) return;
-    if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);        // as the next launch expects it
-    float* wgt = &so[0][0][0];                                       // [16][64] weights of the splits, then [16] maxima and [16] 1 / sums
-    for (int cn = w; cn < nv; cn += W) {
-        const int cc = blockIdx.z * 16 + cn;
-        const size_t r = out_row(cc);
-        const float2 ml = lane < sp.n ? get2(reinterpret_cast<const float*>(sp.part_ml + r * sp.n + lane)) : float2{-INFINITY, 0.f};
-        const float mm = wave_max(ml.x), e = __builtin_amdgcn_exp2f(ml.x - (mm == -INFINITY ? 0.f : mm)), ll = wave_sum(lane < sp.n ? ml.y * e : 0.f);
-        wgt[cn * 64 + lane] = e / ll;
-        if (lane == 0) { wgt[1024 + cn] = mm; wgt[1040 + cn] = 1.f / ll; if (a.ml) a.ml[r] = float2{mm, ll}; }
+    if (sp.n > 1) {
+        unsigned* counter = sp.counters + blockIdx.z * gridDim.y + hkv;
+        if (threadIdx.x == 0) last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)sp.n - 1;
+        __syncthreads();
+        if (!last) return;
+        if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);    // as the next launch expects it
     }
-    __syncthreads();
-    if (sp.n > 1)
+    // everything the first round of either loop needs is asked for before anything is waited for
+    const int tw = threadIdx.x * 2;
+    const bool early = sp.scores && nv == 1 && tw < a.mass_n;
+    float2 s0 = {0.f, 0.f}, in0 = {0.f, 0.f};
+    if (early) {
+        s0 = get2(sp.scores + (size_t)(hkv * G) * sp.scores_ld + tw);
+        in0 = {a.mass_in[(size_t)hkv * a.mass_ld + tw], a.mass_in[(size_t)hkv * a.mass_ld + min(tw + 1, a.mass_n - 1)]};
+    }
+    if (sp.n > 1) {
         for (int j = threadIdx.x; j < nv * (D / 2); j += 64 * W) {
-            const int cn = j / (D / 2), d = (j % (D / 2)) * 2, cc = blockIdx.z * 16 + cn;
-            const size_t r = out_row(cc);
+            const int cn = j / (D / 2), d = (j % (D / 2)) * 2;
+            const size_t r = out_row(blockIdx.z * 16 + cn);
             const float* po = sp.part_o + r * sp.n * D + d;
-            float x = 0.f, y = 0.f;
+            const float* pm = reinterpret_cast<const float*>(sp.part_ml + r * sp.n);
+            float mm = -INFINITY, ll = 0.f, x = 0.f, y = 0.f;
             for (int i0 = 0; i0 < sp.n; i0 += 8) {
-                float2 v[8];
+                float2 v[8], ml[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = get2(po + (size_t)min(i0 + i, sp.n - 1) * D);
+                for (int i = 0; i < 8; ++i) { const int k = min(i0 + i, sp.n - 1); ml[i] = get2(pm + 2 * k); v[i] = get2(po + (size_t)k * D); }
+                float mn = mm;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float e = i0 + i < sp.n ? wgt[cn * 64 + i0 + i] : 0.f;
-                    x = i0 + i < sp.n ? fmaf(v[i].x, e, x) : x; y = i0 + i < sp.n ? fmaf(v[i].y, e, y) : y;
-                }
+                for (int i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
+                const float mu = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(mm - mu);
+                x *= al; y *= al; ll *= al; mm = mn;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i0 + i < sp.n) {
+                        const float e = __builtin_amdgcn_exp2f(ml[i].x - mu);
+                        x = fmaf(v[i].x, e, x); y = fmaf(v[i].y, e, y); ll = fmaf(ml[i].y, e, ll);
+                    }
             }
-            *reinterpret_cast<float2*>(a.out + r * D + d) = float2{x, y};
+            *reinterpret_cast<float2*>(a.out + r * D + d) = float2{x / ll, y / ll};
+            if (d == 0) { fin[0][cn] = mm; fin[1][cn] = 1.f / ll; if (a.ml) a.ml[r] = float2{mm, ll}; }
         }
+        __syncthreads();
+    }
     if (sp.scores)                                                   // one row: columns are the heads of the group
-        for (int t2 = threadIdx.x * 2; t2 < a.mass_n; t2 += 128 * W) {
+        for (int t2 = tw; t2 < a.mass_n; t2 += 128 * W) {
+            const bool have = early && t2 == tw;
+            const size_t at = (size_t)hkv * a.mass_ld + t2;
             float x = 0.f, y = 0.f;
             for (int g = 0; g < nv; ++g) {
-                const float2 s = get2(sp.scores + (size_t)(hkv * G + g) * sp.scores_ld + t2);
-                const float mm = wgt[1024 + g], il = wgt[1040 + g];
-                x = fmaf(__builtin_amdgcn_exp2f(s.x - mm), il, x); y = fmaf(__builtin_amdgcn_exp2f(s.y - mm), il, y);
+                const float2 s = have ? s0 : get2(sp.scores + (size_t)(hkv * G + g) * sp.scores_ld + t2);
+                x = fmaf(__builtin_amdgcn_exp2f(s.x - fin[0][g]), fin[1][g], x); y = fmaf(__builtin_amdgcn_exp2f(s.y - fin[0][g]), fin[1][g], y);
             }
-            const size_t at = (size_t)hkv * a.mass_ld + t2;
-            a.mass_out[at] = a.mass_in[at] + x;
-            if (t2 + 1 < a.mass_n) a.mass_out[at + 1] = a.mass_in[at + 1] + y;
+            a.mass_out[at] = (have ? in0.x : a.mass_in[at]) + x;
+            if (t2 + 1 < a.mass_n) a.mass_out[at + 1] = (have ? in0.y : a.mass_in[at + 1]) + y;
         }
 }
-// Joins many splits of a row and head, a workgroup each: 256 / (D / 4) groups of threads take the splits in turn.
+// After a split that was not joined inside its launch.  The first M H workgroups join a row and head each: 256 / (D / 4) groups of threads take
+// the splits in turn.  The others (one row, scores left behind) count the weights: 512 positions of a K/V head each, with maxima and sums of
+// the group's heads from their parts, so that they need not wait for the join.
 template <int D>
-__global__ __launch_bounds__(256) void kv8_attn_join_kernel(Kv8Attn a, Kv8Split sp) {
+__global__ __launch_bounds__(256) void kv8_attn_finish_kernel(Kv8Attn a, Kv8Split sp) {
     constexpr int R = 256 / (D / 4);
     __shared__ f4 part[R][D / 4];
-    const size_t r = blockIdx.x;
-    const int lane = threadIdx.x & 63, d = threadIdx.x % (D / 4), g = threadIdx.x / (D / 4);
-    const float2 ml = lane < sp.n ? sp.part_ml[r * sp.n + lane] : float2{-INFINITY, 0.f};
-    const float m = wave_max(ml.x), e = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m)), l = wave_sum(lane < sp.n ? ml.y * e : 0.f);
-    f4 sum = f4{0.f, 0.f, 0.f, 0.f};
-    for (int i = g; i < sp.n; i += R) {
-        const float ei = __shfl(e, i);
-        const f4 v = reinterpret_cast<const f4*>(sp.part_o + (r * sp.n + i) * D)[d];
+    __shared__ float fin[2][16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    auto stats = [&](size_t r, float& e) {                           // the row's maximum and sum; e: this lane's split's share
+        const float2 ml = lane < sp.n ? sp.part_ml[r * sp.n + lane] : float2{-INFINITY, 0.f};
+        const float m = wave_max(ml.x);
+        e = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m));
+        return float2{m, wave_sum(lane < sp.n ? ml.y * e : 0.f)};
+    };
+    if (blockIdx.x < (unsigned)(a.M * a.c.H)) {
+        const size_t r = blockIdx.x;
+        const int d = threadIdx.x % (D / 4), g = threadIdx.x / (D / 4);
+        float e;
+        const float2 ml = stats(r, e);
+        f4 sum = f4{0.f, 0.f, 0.f, 0.f};
+        for (int i = g; i < sp.n; i += R) {
+            const float ei = __shfl(e, i);
+            const f4 v = reinterpret_cast<const f4*>(sp.part_o + (r * sp.n + i) * D)[d];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] = fmaf(v[k], ei, sum[k]);
-    }
-    part[g][d] = sum;
-    __syncthreads();
-    if (threadIdx.x < D / 4) {
-        sum = part[0][d];
-#pragma unroll
-        for (int i = 1; i < R; ++i) sum += part[i][d];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] = sum[k] / l;
-        reinterpret_cast<f4*>(a.out + r * D)[d] = sum;
-    }
-    if (threadIdx.x == 0 && a.ml) a.ml[r] = float2{m, l};
-}
-// mass_out = mass_in + the softmax weights of one row, from the scores the attention left: 1024 positions a workgroup
-__global__ __launch_bounds__(256) void kv8_mass_scores_kernel(Kv8Attn a, Kv8Split sp) {
-    const int G = a.c.H / a.c.Hkv, hkv = blockIdx.y;
-    for (int t = blockIdx.x * 1024 + threadIdx.x, i = 0; i < 4 && t < a.mass_n; ++i, t += 256) {
-        float sum = 0.f;
-        for (int g = 0; g < G; ++g) {
-            const float2 ml = a.ml[hkv * G + g];
-            sum += __builtin_amdgcn_exp2f(sp.scores[(size_t)(hkv * G + g) * sp.scores_ld + t] - ml.x) / ml.y;
+            for (int k = 0; k < 4; ++k) sum[k] = fmaf(v[k], ei, sum[k]);
         }
-        a.mass_out[(size_t)hkv * a.mass_ld + t] = a.mass_in[(size_t)hkv * a.mass_ld + t] + sum;
+        part[g][d] = sum;
+        __syncthreads();
+        if (threadIdx.x < D / 4) {
+            sum = part[0][d];
+#pragma unroll
+            for (int i = 1; i < R; ++i) sum += part[i][d];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k] = sum[k] / ml.y;
+            reinterpret_cast<f4*>(a.out + r * D)[d] = sum;
+        }
+        if (threadIdx.x == 0 && a.ml) a.ml[r] = ml;
+        return;
     }
+    const int chunks = (a.mass_n + 511) / 512, b = blockIdx.x - a.M * a.c.H, hkv = b / chunks, t = (b % chunks) * 512 + threadIdx.x * 2, G = a.c.H / a.c.Hkv;
+    float2 s[4];
+    auto load = [&](int g0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = *reinterpret_cast<const float2*>(sp.scores + (size_t)(hkv * G + min(g0 + i, G - 1)) * sp.scores_ld + t);
+    };
+    if (t < a.mass_n) load(0);
+    for (int g = w; g < G; g += 4) {
+        float e;
+        const float2 ml = stats((size_t)hkv * G + g, e);
+        if (lane == 0) { fin[0][g] = ml.x; fin[1][g] = 1.f / ml.y; }
+    }
+    __syncthreads();
+    if (t >= a.mass_n) return;
+    const size_t at = (size_t)hkv * a.mass_ld + t;
+    const float in0 = a.mass_in[at], in1 = a.mass_in[(size_t)hkv * a.mass_ld + min(t + 1, a.mass_n - 1)];
+    float x = 0.f, y = 0.f;
+    for (int g0 = 0; g0 < G; g0 += 4) {
+        if (g0 > 0) load(g0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (g0 + i < G) {
+                x = fmaf(__builtin_amdgcn_exp2f(s[i].x - fin[0][g0 + i]), fin[1][g0 + i], x);
+                y = fmaf(__builtin_amdgcn_exp2f(s[i].y - fin[0][g0 + i]), fin[1][g0 + i], y);
+            }
+    }
+    a.mass_out[at] = in0 + x;
+    if (t + 1 < a.mass_n) a.mass_out[at + 1] = in1 + y;
 }
 
 // ---------------------------------------------------------------- attention of many rows: f16 matrix instructions, tiles shared through LDS
@@ -1148,14 +1227,15 @@ template <int D, int W> static void attn_split(const Kv8Attn& a, const Kv8Split&
 }
 hipError_t launch_kv8_attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t st) {
     switch (a.c.D) {
-        case 64: if (sp.waves == 8) attn_split<64, 8>(a, sp, st); else attn_split<64, 4>(a, sp, st); break;
-        case 128: if (sp.waves == 8) attn_split<128, 8>(a, sp, st); else if (sp.waves == 2) attn_split<128, 2>(a, sp, st); else attn_split<128, 4>(a, sp, st); break;
-        case 256: attn_split<256, 4>(a, sp, st); break;
+        case 64: attn_split<64, kv8_split_waves(64)>(a, sp, st); break;
+        case 128: attn_split<128, kv8_split_waves(128)>(a, sp, st); break;
+        case 256: attn_split<256, kv8_split_waves(256)>(a, sp, st); break;
         default: return hipErrorInvalidValue;
     }
-    if (sp.counters) return hipGetLastError();
-    if (sp.n > 1) KV8_BY_DIM(a.c.D, hipLaunchKernelGGL(kv8_attn_join_kernel<kD>, dim3(a.M * a.c.H), dim3(256), 0, st, a, sp));
-    if (sp.scores) hipLaunchKernelGGL(kv8_mass_scores_kernel, dim3((a.mass_n + 1023) / 1024, a.c.Hkv), dim3(256), 0, st, a, sp);
+    if (!sp.counters && sp.n > 1) {
+        const unsigned mass = sp.scores ? (unsigned)((a.mass_n + 511) / 512 * a.c.Hkv) : 0u;
+        KV8_BY_DIM(a.c.D, hipLaunchKernelGGL(kv8_attn_finish_kernel<kD>, dim3(a.M * a.c.H + mass), dim3(256), 0, st, a, sp));
+    }
     return hipGetLastError();
 }
 

@@ -9,7 +9,7 @@ static const int kKv8Block = 16;      // positions that share one K scale and on
 static const int kKv8Tile = 64;       // positions one step of the split attention kernel takes
 static const int kKv8Pad = 128;       // a cache holds whole multiples of this many positions: no kernel's step reads behind it
 static const int kKv8SplitRows = 8192; // rows x splits whose parts the workspace holds
-static const int kKv8Counters = 8192;  // column groups x K/V heads that can be joined inside the launch
+static const int kKv8Groups = 512;    // column groups x K/V heads up to which the positions are split (and counters there are)
 static const int kKv8RowSlab = 2048;  // prompt rows one attention launch takes (sizes the per-row statistics)
 
 // Device memory of one cache.  n_blk = blocks per head, a multiple of 8 (kKv8Pad).
@@ -40,9 +40,9 @@ struct Kv8Attn {
 };
 
 // Few rows over a long axis: the positions are cut into n <= 64 parts of whole tiles.  With counters the last workgroup of a column group joins
-// the parts (and counts the weights), otherwise launches of their own do.
+// the parts (and counts the weights), otherwise a second launch does where n > 1.  Scores without counters need n > 1.
 struct Kv8Split {
-    int n, waves;                     // parts; waves of a workgroup, 4 or 8
+    int n;
     bool stream;                      // the codes are read past the caches
     float* part_o;                    // [M H][n][D]
     float2* part_ml;                  // [M H][n]
@@ -50,6 +50,7 @@ struct Kv8Split {
     int64_t scores_ld;
     unsigned* counters;               // one per column group and K/V head, zero between launches; or null
 };
+constexpr int kv8_split_waves(int D) { return D == 256 ? 4 : 8; }      // of a workgroup, a tile each in turn; one workgroup fills a CU's registers (two, D = 64)
 
 hipError_t launch_kv8_append(const Kv8View& c, const float* k, const float* v, int64_t pos, int64_t n, hipStream_t st);
 hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_out, float* v_out, hipStream_t st);
