@@ -231,6 +231,37 @@ def test_nan_reaches_only_rows_that_see_it(thk, ctx, what):
         assert np.all(np.abs(m - em) <= tm)
 
 
+@pytest.mark.parametrize("H,Hkv,D,T", [(8, 4, 64, 150), (32, 32, 128, 300), (64, 64, 64, 200), (24, 8, 256, 120)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_odd_queries(thk, ctx, H, Hkv, D, T, bad):
+    """A query that is not finite gives NaN in its own row and on the weights of the positions it sees, nowhere else; a query of zeros gives the mean."""
+    rng = np.random.default_rng(T + D)
+    p = Pair(thk, ctx, T, H, Hkv, D)
+    p.append(rows(rng, T, Hkv, D), 0)
+    q = rng.standard_normal((T, H, D)).astype(np.float32)
+    r, h, z = T // 2, H - 2, T - 3
+    q[z] = 0
+    mass = rng.random((Hkv, T)).astype(np.float32)
+    clean = q.copy()
+    q[r, h, 5] = bad
+    eo, em, to, tm = attention(p.ref.values(0, T), clean, 0, mass)
+    out, m = p.attend(q, 0, mass)
+    nan = np.zeros((T, H), bool)
+    nan[r, h] = True
+    assert np.array_equal(np.isnan(out).any(2), nan) and np.isnan(out[r, h]).all()
+    assert np.all((np.abs(out - eo) <= to)[~nan])
+    touched = np.zeros((Hkv, T), bool)
+    touched[h * Hkv // H, :r + 1] = True
+    assert np.array_equal(np.isnan(m), touched)
+    late = np.zeros((Hkv, T), bool)
+    late[:, r + 1:] = True
+    assert np.all((np.abs(m - em) <= tm)[late | ~touched])
+    for t in (r, z):                                               # the same rows as single tokens
+        out, m = p.attend(q[t:t + 1], t, mass, decode=True)
+        assert np.array_equal(np.isnan(out[0]).any(1), nan[t]) and np.all((np.abs(out[0] - eo[t]) <= to[t])[~nan[t]])
+        assert np.array_equal(np.isnan(m), touched & nan.any(1)[t]) and np.all(m[:, t + 1:] == 7.0)
+
+
 def test_garbage_behind_the_last_position(thk, ctx):
     """Positions at and after T hold infinities and NaN: no row reads them."""
     rng = np.random.default_rng(14)

@@ -401,18 +401,13 @@ static const float kLog2e = 1.44269504088896340736f;      // scores carry log2(e
 // out_n = sum_t p_nt v_t with p = softmax(q_n . k_t), for up to 16 (row, head) columns n that read one K/V head.  Both products run on
 // v_mfma_i32_16x16x64_i8 with the cache's codes as they are - no conversion - and the f32 operand (q, then the weights) as a fixed-point
 // number of three balanced base-256 digits: x = d2 2^16 + d1 2^8 + d0, each digit an i8 operand of its own product, the three i32 sums
-// exact.  q is fixed relative to its column's largest entry (23 bits), the weights p * v_scale relative to the largest of their column
+// exact.  q is fixed relative to its column's largest entry (23 bits with the sign), the weights p * v_scale relative to the largest of their column
 // in the tile of 64 positions (a power of two, 21 to 22 bits): errors stay at f32's own.
 // Operand layout (A: row = lane % 16, B: column = lane % 16, both 16 consecutive k per lane of chunk lane / 16; result: column lane % 16,
 // rows 4 (lane / 16) + i).  The k order is free as long as A and B share it, and the row order of the first product is chosen so that
 // lane chunk c ends up with the scores of the 16 positions of block c: then one K scale and one V scale per lane serve a whole tile, and
 // the second product's B operand is what the lane already holds - no exchange between lanes.
 typedef int i4 __attribute__((ext_vector_type(4)));
-#ifdef KV8_NT
-__device__ __forceinline__ i4 LD(const void* p) { return __builtin_nontemporal_load(reinterpret_cast<const i4*>(p)); }
-#else
-__device__ __forceinline__ i4 LD(const void* p) { return *reinterpret_cast<const i4*>(p); }
-#endif
 struct U2 { unsigned a, b; };
 // Between them, a and b hold a value and that of the lane 16 (32) away, in every lane.  The swap works on two registers: the empty asm keeps
 // the compiler from giving it the same one twice, which would leave the value where it is.
@@ -444,15 +439,15 @@ __device__ __forceinline__ float chunks_sum(float v) {
     r = pair32(as_u(as_f(r.a) + as_f(r.b)));
     return as_f(r.a) + as_f(r.b);
 }
-// Four numbers whose low two bytes are digits plus 128 (x + 0x8080 for x >= 0, x + 0x808080 with SIGNED: then the third byte too): their
-// digits, four to a word.
+// Four numbers x + 0x8080, with SIGNED x + 0x408080, |x| < 0x3F7F80: their digits, four to a word.
 template <bool SIGNED>
 __device__ __forceinline__ void pack_digits(unsigned e0, unsigned e1, unsigned e2, unsigned e3, int& d2, int& d1, int& d0) {
     const unsigned a = __builtin_amdgcn_perm(e1, e0, 0x05040100u), b = __builtin_amdgcn_perm(e3, e2, 0x05040100u);     // bytes: e0.0 e0.1 e1.0 e1.1
     const unsigned u = __builtin_amdgcn_perm(e1, e0, 0x0C0C0602u), w = __builtin_amdgcn_perm(e3, e2, 0x06020C0Cu);
     d0 = (int)(__builtin_amdgcn_perm(b, a, 0x06040200u) ^ 0x80808080u);
     d1 = (int)(__builtin_amdgcn_perm(b, a, 0x07050301u) ^ 0x80808080u);
-    d2 = (int)(SIGNED ? (u | w) ^ 0x80808080u : u | w);
+    d2 = (int)(u | w);
+    if (SIGNED) { const unsigned t = (u | w) ^ 0x40404040u; d2 = (int)(t | (t & 0x40404040u) << 1); }      // bytes 0 .. 127, less 64
 }
 __device__ __forceinline__ float join_digits(int i2, int i1, int i0) { return fmaf((float)i2, 65536.f, (float)(i1 * 256 + i0)); }   // |i1| <= 256 * 2^14: no overflow
 
@@ -473,18 +468,18 @@ __device__ __forceinline__ float digits_of(const f4 (&x)[N], Max column_max, Put
     m = column_max(m);
     const float amax = as_f(m);
     const bool some = amax >= 0x1p-100f;                                   // also false for NaN
-    const float inv = some && m < 0x7F800000u ? 8355000.f / amax : 0.f;    // below 127 (2^16 + 2^8 + 1), the largest sum of three balanced digits, by more than the roundings
+    const float inv = some && m < 0x7F800000u ? 4161000.f / amax : 0.f;    // x + 2^22 + 0x8080 is the mantissa of the sum below: it has to stay under 2^23
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         unsigned e[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = (unsigned)((int)rintf(x[i][j] * inv) + 0x808080);
+        for (int j = 0; j < 4; ++j) e[j] = as_u(fmaf(x[i][j], inv, 12615808.f));
         int d2, d1, d0;
         pack_digits<true>(e[0], e[1], e[2], e[3], d2, d1, d0);
         put(i, d2, d1, d0);
     }
     if (m >= 0x7F800000u) return as_f(0x7FC00000u);                        // a query that is not finite: every score is NaN
-    return some ? amax / 8355000.f : 0.f;
+    return some ? amax / 4161000.f : 0.f;
 }
 template <int D>
 __device__ __forceinline__ float q_digits(const f4 (&x)[D / 16], i4 (&qd)[3][D / 64]) {
@@ -894,16 +889,19 @@ __device__ __forceinline__ int xcd_order(int id, int n) {
     return x * q + (x < r ? x : r) + id / 8;
 }
 
-template <int D, int NC>
-__global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int blocks, float scale) {
+template <int D, int NC, int S>
+__global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, int blocks, float scale) {
     constexpr int ST = D / 32, NG = D / 16, KF = 4 * ST, VF = 2 * NG, PIECES = (D / 64 * 4 + NG) / 4;      // f16 fragments of a tile; 16-byte pieces a thread stages
     extern __shared__ __align__(16) char smem[];
-    hf8* frag = reinterpret_cast<hf8*>(smem);                              // [2][KF + VF][64]: K fragments (group, step), V fragments (dimensions, half)
     const Kv8View& c = a.c;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, ch = lane >> 4;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6 & 3, grp = S > 1 ? threadIdx.x >> 8 : 0, n = lane & 15, ch = lane >> 4;
+    hf8* frag = reinterpret_cast<hf8*>(smem) + grp * (2 * (KF + VF) * 64);   // [2][KF + VF][64]: K fragments (group, step), V fragments (dimensions, half)
     const int id = xcd_order(blockIdx.x, gridDim.x), hkv = id / blocks, blk = blocks - 1 - id % blocks;       // longest rows first
-    const int G = c.H / c.Hkv, cols = a.M * G, col0 = blk * 64 * NC, wcol0 = col0 + w * 16 * NC;
-    const int T = a.n_past + (min(col0 + 64 * NC, cols) - 1) / G + 1, tiles = (T + kKv8Tile - 1) / kKv8Tile;
+    // S = 2: the columns are half a block from the front and half from the back, so that all workgroups have alike to do, and each SIMD has
+    // a wave of either half
+    const int G = c.H / c.Hkv, cols = a.M * G, set = (w + 2 * grp) & 3, half = set < 2 ? 2 * blocks - 1 - blk : blk;
+    const int wcol0 = S > 1 ? half * 32 * NC + (set & 1) * 16 * NC : (blk * 4 + w) * 16 * NC, end = S > 1 ? (2 * blocks - blk) * 32 * NC : (blk + 1) * 64 * NC;
+    const int T = a.n_past + (min(end, cols) - 1) / G + 1, tiles = (T + kKv8Tile - 1) / kKv8Tile;
     const int wrow0 = wcol0 / G, wrow1 = (min(wcol0 + 16 * NC, cols) - 1) / G;                             // rows this wave holds (none: wcol0 >= cols)
     const int8_t* kb = c.k + ((size_t)hkv * c.n_blk * kKv8Block + 16 * (n >> 2) + (n & 3)) * D + ch * 16;
     const int8_t* vb = c.v + (((size_t)hkv * c.n_blk + ch) * D + n) * 16;
@@ -929,7 +927,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int bl
             f[(2 * p + 1) * 64] = h.b;
         }
     };
-    fetch(0);
+    fetch(grp);                                                            // tiles to a multiple of S exist in the cache; those behind T are skipped
     hf8 qh[NC][ST], ql[NC][ST];
     float qf[NC], m[NC], l[NC];
     int ref[NC], lim[NC];
@@ -945,17 +943,18 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int bl
         for (int g = 0; g < NG; ++g) o[k][g] = f4{0.f, 0.f, 0.f, 0.f};
     }
     stage(0);
-    float ks = ksb[0], vs = vsb[0];
+    float ks = ksb[grp * 4], vs = vsb[grp * 4];
     asm("" : "+v"(ks), "+v"(vs));                                          // here, not in the loop, is where they are waited for
     __syncthreads();
     // One tile.  `more` is a constant in each of its two uses: with a branch around the loads the compiler would wait for all of them wherever
     // it waits for any.
-    auto step = [&](int t, auto more_) {
+    auto step = [&](int it, auto more_) {
         constexpr bool more = decltype(more_)::value;
+        const int t = it * S + grp;
         float ksn = 0.f, vsn = 0.f;
-        if (more) { fetch(t + 1); ksn = ksb[(size_t)(t + 1) * 4]; vsn = vsb[(size_t)(t + 1) * 4]; }
+        if (more) { fetch(t + S); ksn = ksb[(size_t)(t + S) * 4]; vsn = vsb[(size_t)(t + S) * 4]; }
         if (wcol0 < cols && t * kKv8Tile <= a.n_past + wrow1) {             // some row of this wave sees the tile
-            const hf8* kf_ = frag + (size_t)(t & 1) * (KF + VF) * 64 + lane;
+            const hf8* kf_ = frag + (size_t)(it & 1) * (KF + VF) * 64 + lane;
             const hf8* vf_ = kf_ + KF * 64;
             // both products: the fragments of the next step are read while the present one's matrix instructions run, and 2 NC sums
             // take turns, so that each finds its predecessor done
@@ -1054,10 +1053,36 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Kv8Attn a, int bl
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (more) { stage((t + 1) & 1); ks = ksn; vs = vsn; __syncthreads(); }
+        if (more) { stage((it + 1) & 1); ks = ksn; vs = vsn; __syncthreads(); }
     };
-    for (int t = 0; t + 1 < tiles; ++t) step(t, std::true_type{});
-    step(tiles - 1, std::false_type{});
+    const int steps = (tiles + S - 1) / S;
+    for (int it = 0; it + 1 < steps; ++it) step(it, std::true_type{});
+    step(steps - 1, std::false_type{});
+    if (S > 1) {                                                           // the second group's sums join the first's
+        f4* so = reinterpret_cast<f4*>(smem);                              // [NC][NG + 1][256]
+        const int tid = set * 64 + lane;
+        __syncthreads();                                                   // the fragments have been read
+        if (grp == 1) {
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) so[(k * (NG + 1) + g) * 256 + tid] = o[k][g];
+                so[(k * (NG + 1) + NG) * 256 + tid] = f4{m[k], l[k], (float)ref[k], 0.f};
+            }
+        }
+        __syncthreads();
+        if (grp == 1) return;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            const f4 st1 = so[(k * (NG + 1) + NG) * 256 + tid];
+            const float mn = fmaxf(m[k], st1[0]), mu = mn == -INFINITY ? 0.f : mn, a0 = __builtin_amdgcn_exp2f(m[k] - mu), a1 = __builtin_amdgcn_exp2f(st1[0] - mu);
+            const int r1 = (int)st1[2], rn = max(ref[k], r1);
+            const float f0 = ldexpf(a0, max(ref[k] - rn, -2000)), f1 = ldexpf(a1, max(r1 - rn, -2000));
+#pragma unroll
+            for (int g = 0; g < NG; ++g) o[k][g] = o[k][g] * f0 + so[(k * (NG + 1) + g) * 256 + tid] * f1;
+            l[k] = fmaf(st1[1], a1, l[k] * a0); m[k] = mn; ref[k] = rn;
+        }
+    }
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
         const int col = wcol0 + 16 * k + n;
@@ -1108,7 +1133,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_mass_tile_kernel
         const float qf = q_digits<D>(x, qd) * scale, top = ml.x, inv = 1.f / ml.y;
         load(min(c0 + 16 * W, cols - 1));                                      // without a branch: the next ones, or any
         const int row = min(c0 + n, cols - 1) / G, lim = c0 + n < cols ? a.n_past + row : -1;
+        const bool edge = __any(tile * kKv8Tile + kKv8Tile - 1 > lim);
         const float kf = pos <= lim && qf * ks != 0.f ? qf * ks : 1.f;     // a block this column does not see: no factor that could be NaN
+        float p[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             i4 acc[3];
@@ -1119,10 +1146,14 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_mass_tile_kernel
                 for (int kc = 0; kc < KC; ++kc) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[g][kc], qd[d][kc], acc[d], 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(join_digits(acc[2][i], acc[1][i], acc[0][i]), kf, -top)) * inv;
-                sum[4 * g + i] += pos + 4 * g + i <= lim ? p : 0.f;
-            }
+            for (int i = 0; i < 4; ++i) p[4 * g + i] = __builtin_amdgcn_exp2f(fmaf(join_digits(acc[2][i], acc[1][i], acc[0][i]), kf, -top));
+        }
+        if (edge) {                                                        // a row of NaN weights must not reach positions it does not see
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[i] += pos + i <= lim ? p[i] * inv : 0.f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[i] = fmaf(p[i], inv, sum[i]);
         }
     }
 #pragma unroll
@@ -1192,20 +1223,29 @@ hipError_t launch_kv8_move(const Kv8View& src, const Kv8View& dst, int n_keep, c
     KV8_BY_DIM(src.D, hipLaunchKernelGGL(kv8_move_kernel<kD>, grid, dim3(256), 0, st, src, dst, n_keep, kept));
     return hipGetLastError();
 }
-template <int D, int NC> static hipError_t attn_tile(const Kv8Attn& a, hipStream_t st) {
-    constexpr size_t lds = (size_t)2 * (4 * (D / 32) + 2 * (D / 16)) * 64 * 16;
+template <int D, int NC, int S> static hipError_t attn_tile(const Kv8Attn& a, hipStream_t st) {
+    constexpr size_t lds = (size_t)S * 2 * (4 * (D / 32) + 2 * (D / 16)) * 64 * 16;
     const int cols = a.M * (a.c.H / a.c.Hkv), blocks = (cols + 64 * NC - 1) / (64 * NC);
-    const hipError_t e = lds_opt_in(kv8_attn_tile_kernel<D, NC>, lds);
+    const hipError_t e = lds_opt_in(kv8_attn_tile_kernel<D, NC, S>, lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((kv8_attn_tile_kernel<D, NC>), dim3(blocks * a.c.Hkv), dim3(256), lds, st, a, blocks, kLog2e / sqrtf((float)D));
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<D, NC, S>), dim3(blocks * a.c.Hkv), dim3(256 * S), lds, st, a, blocks, kLog2e / sqrtf((float)D));
     return hipGetLastError();
 }
-hipError_t launch_kv8_attn_tile(const Kv8Attn& a, hipStream_t st) {
-    // 32 columns a wave halve the LDS reads of 16, once there are enough workgroups for every CU to hold two
+template <int D> static hipError_t attn_tile(const Kv8Attn& a, hipStream_t st) {
+    // 32 columns a wave halve the LDS reads of 16, once there are enough workgroups for every CU to hold two; where there is at most one workgroup
+    // a CU, a second group of waves takes every other tile.
     const int64_t cols = (int64_t)a.M * (a.c.H / a.c.Hkv);
-    if (a.c.D == 256) return attn_tile<256, 1>(a, st);
-    if ((cols + 127) / 128 * a.c.Hkv >= 384) return a.c.D == 64 ? attn_tile<64, 2>(a, st) : attn_tile<128, 2>(a, st);
-    return a.c.D == 64 ? attn_tile<64, 1>(a, st) : attn_tile<128, 1>(a, st);
+    if ((cols + 127) / 128 * a.c.Hkv >= 384) return attn_tile<D, 2, 1>(a, st);
+    if ((cols + 63) / 64 * a.c.Hkv <= 256) return attn_tile<D, 1, 2>(a, st);
+    return attn_tile<D, 1, 1>(a, st);
+}
+hipError_t launch_kv8_attn_tile(const Kv8Attn& a, hipStream_t st) {
+    switch (a.c.D) {
+        case 64: return attn_tile<64>(a, st);
+        case 128: return attn_tile<128>(a, st);
+        case 256: return attn_tile<256, 1, 1>(a, st);                      // one group's tiles fill the LDS
+        default: return hipErrorInvalidValue;
+    }
 }
 template <int D> static hipError_t mass_tile(const Kv8Attn& a, hipStream_t st) {
     const int tiles = (a.n_past + a.M + kKv8Tile - 1) / kKv8Tile;
