@@ -69,6 +69,8 @@ TINY_Q1 = ModelShape(n_vocab=32000, n_embd=512, n_mult=256, n_head=8, n_layer=2,
 
 
 def _ptr(x) -> int:
+    if type(x) is int:
+        return x
     if x is None:
         return 0
     if isinstance(x, Buffer):
@@ -242,6 +244,10 @@ class KvCache8:
         h = C.c_void_p()
         ctx.check(ctx.lib.thk_kv8_create(ctx.h, n_ctx, n_head, n_head_kv, head_dim, C.byref(h)), "thk_kv8_create")
         self.h = h
+        # the calls of a decode loop are short (a launch or two): they are bound once
+        lib = ctx.lib
+        self._append, self._read, self._decode, self._prefill, self._evict = (
+            lib.thk_kv8_append, lib.thk_kv8_read, lib.thk_kv8_attn_decode, lib.thk_kv8_attn_prefill, lib.thk_kv8_evict)
 
     def close(self):
         if getattr(self, "h", None) and getattr(self.ctx, "h", None):
@@ -260,23 +266,33 @@ class KvCache8:
 
     def append(self, k, v, pos: int, n_tok: int):
         """Positions [pos, pos + n_tok) from k, v f32 [n_tok, n_head_kv, head_dim]."""
-        self.ctx.check(self.ctx.lib.thk_kv8_append(self.h, _ptr(k), _ptr(v), pos, n_tok), "thk_kv8_append")
+        rc = self._append(self.h, _ptr(k), _ptr(v), pos, n_tok)
+        if rc:
+            self.ctx.check(rc, "thk_kv8_append")
 
     def read(self, pos: int, n_tok: int, k_out, v_out):
         """The values of positions [pos, pos + n_tok) as f32 [n_tok, n_head_kv, head_dim]; either output may be None."""
-        self.ctx.check(self.ctx.lib.thk_kv8_read(self.h, pos, n_tok, _ptr(k_out), _ptr(v_out)), "thk_kv8_read")
+        rc = self._read(self.h, pos, n_tok, _ptr(k_out), _ptr(v_out))
+        if rc:
+            self.ctx.check(rc, "thk_kv8_read")
 
     def attn_decode(self, q, T: int, out, mass_in=None, mass_out=None):
         """One query token over the first T positions; mass_out = mass_in + its softmax weights (f32 [n_head_kv, n_ctx])."""
-        self.ctx.check(self.ctx.lib.thk_kv8_attn_decode(self.h, _ptr(q), T, _ptr(mass_in), _ptr(mass_out), _ptr(out)), "thk_kv8_attn_decode")
+        rc = self._decode(self.h, _ptr(q), T, _ptr(mass_in), _ptr(mass_out), _ptr(out))
+        if rc:
+            self.ctx.check(rc, "thk_kv8_attn_decode")
 
     def attn_prefill(self, q, n_past: int, M: int, out, mass_in=None, mass_out=None):
         """M query rows, row i over positions <= n_past + i."""
-        self.ctx.check(self.ctx.lib.thk_kv8_attn_prefill(self.h, _ptr(q), n_past, M, _ptr(mass_in), _ptr(mass_out), _ptr(out)), "thk_kv8_attn_prefill")
+        rc = self._prefill(self.h, _ptr(q), n_past, M, _ptr(mass_in), _ptr(mass_out), _ptr(out))
+        if rc:
+            self.ctx.check(rc, "thk_kv8_attn_prefill")
 
     def evict(self, dst: "KvCache8", T: int, n_keep: int, n_sink: int, n_recent: int, mass_in, mass_out, kept):
         """Every K/V head's n_keep positions (first n_sink, last n_recent, heaviest others) into dst; kept: dev int32 [n_head_kv, n_keep]."""
-        self.ctx.check(self.ctx.lib.thk_kv8_evict(self.h, T, n_keep, n_sink, n_recent, _ptr(mass_in), dst.h, _ptr(mass_out), _ptr(kept)), "thk_kv8_evict")
+        rc = self._evict(self.h, T, n_keep, n_sink, n_recent, _ptr(mass_in), dst.h, _ptr(mass_out), _ptr(kept))
+        if rc:
+            self.ctx.check(rc, "thk_kv8_evict")
 
 
 class Model:
