@@ -32,7 +32,7 @@ int64_t tun(thk_ctx*, const char*) { return 0; }
 namespace thk {
 hipError_t launch_kv8_append(const Kv8View&, const float*, const float*, int64_t pos, int64_t n, hipStream_t) { note("append %lld %lld", (long long)pos, (long long)n); return launched(); }
 hipError_t launch_kv8_read(const Kv8View&, int64_t pos, int64_t n, float*, float*, hipStream_t) { note("read %lld %lld", (long long)pos, (long long)n); return launched(); }
-hipError_t launch_kv8_select(int Hkv, int T, int keep, int sink, int recent, const float*, int64_t li, float*, int64_t lo, int32_t*, hipStream_t) {
+hipError_t launch_kv8_select(int Hkv, int T, int keep, int sink, int recent, const float*, int64_t li, float*, int64_t lo, int32_t*, unsigned*, int64_t, hipStream_t) {
     note("select %d %d %d %d %d %lld %lld", Hkv, T, keep, sink, recent, (long long)li, (long long)lo); return launched();
 }
 hipError_t launch_kv8_move(const Kv8View&, const Kv8View&, int keep, const int32_t*, hipStream_t) { note("move %d", keep); return launched(); }

@@ -191,7 +191,8 @@ extern "C" int thk_kv8_evict(thk_kv8* src, int64_t T, int64_t n_keep, int64_t n_
     REQUIRE(ctx, aligned16(mass_in) && aligned16(mass_out) && aligned16(kept), "thk_kv8_evict: pointers must be 16-byte aligned");
     DeviceScope dev(ctx->device);
     HIPCHK(ctx, dev.err);
-    HIPCHK(ctx, launch_kv8_select(src->view.Hkv, (int)T, (int)n_keep, (int)n_sink, (int)n_recent, mass_in, src->n_ctx, mass_out, dst->n_ctx, kept, ctx->stream));
+    HIPCHK(ctx, launch_kv8_select(src->view.Hkv, (int)T, (int)n_keep, (int)n_sink, (int)n_recent, mass_in, src->n_ctx, mass_out, dst->n_ctx, kept,
+                                  reinterpret_cast<unsigned*>(src->part_o), (int64_t)kKv8SplitRows * src->view.D, ctx->stream));
     HIPCHK(ctx, launch_kv8_move(src->view, dst->view, (int)n_keep, kept, ctx->stream));
     return THK_OK;
 }

@@ -2,6 +2,7 @@
 // Layout: thk_kv8.hpp.  All sums, softmax statistics and scales are f32; the codes are the only 8-bit values.
 #include "thk_device.hpp"
 #include "thk_kv8.hpp"
+#include <algorithm>
 #include <type_traits>
 
 namespace thk {
@@ -171,13 +172,11 @@ __device__ __forceinline__ unsigned mass_key(float x) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float key_mass(unsigned k) { return as_f(k == 1u ? 0x7FC00000u : (k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }
-// One workgroup per K/V head: the n_keep largest keys by radix selection, ties to the lowest position, then the kept positions in ascending order.
-//   W waves; thread t takes positions 4 t .. 4 t + 3 of every 256 W.  With N > 0 (T <= 64 W N) their N keys stay in LDS, else every pass reads
-//   the weights again, 64 a thread at a time.  (Registers would hold them too, but loops over them have to be unrolled, and then spill.)
-//   BITS a pass, histograms in LDS in two interleaved copies by lane (the weights' leading bits take few values, and copies in one bank
-//   would not help); thread t sums the buckets of one stretch, heaviest first.
+// The n_keep largest keys of a head by radix selection, ties to the lowest position, then the kept positions in ascending order.
+//   W waves; thread t takes positions 4 t .. 4 t + 3 of every 256 W.
+//   Histograms in LDS, in interleaved copies by lane (the weights' leading bits take few values, and copies in one bank would not help);
+//   thread t sums the buckets of one stretch, heaviest first.
 //   What stays is one ballot per 64 keys; the ballots' bit counts, summed up over waves, say where each thread's kept positions go.
-// What bounds it is one CU's instruction issue, so small sets take 4 waves instead of 16.
 template <int W> __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* sm, unsigned* total) {     // exclusive prefix sum over 64 W threads; sm: W words
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     unsigned s = v;
@@ -192,123 +191,87 @@ template <int W> __device__ __forceinline__ unsigned block_scan(unsigned v, unsi
     *total = all;
     return before + s - v;
 }
-template <int W, int N, int BITS>
-__global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, int n_sink, int n_recent, const float* __restrict__ mass_in, int64_t ld_in,
-                                                            float* __restrict__ mass_out, int64_t ld_out, int32_t* __restrict__ kept) {
-    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
-    constexpr int Q = (N > 0 ? N : 64) / 4, R = 2, B = 1 << BITS, PT = (B + 64 * W - 1) / (64 * W);     // groups of four a thread and sweep; copies; buckets; buckets a thread
-    __shared__ unsigned hist[B * R], sm[W], pick[3], cnt[Q * W];
-    extern __shared__ __align__(16) char smem[];
-    uint4* keys = reinterpret_cast<uint4*>(smem);                          // [Q][64 W]
-    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, lo = n_sink, hi = T - n_recent;
-    const float* mass = mass_in + (size_t)h * ld_in;
-    unsigned need = (unsigned)n_keep, prefix = 0, same = 0;                // of the `same` positions whose key starts with prefix, the `need` heaviest stay
-    auto load4 = [&](int t, unsigned (&k)[4]) {
+struct Weights {                                                           // of one head; positions outside [lo, hi) stay, positions from end on do not exist
+    const float* mass;
+    int lo, hi, end;
+    __device__ __forceinline__ void load4(int t, unsigned (&k)[4]) const {
+        typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
         f4 v;
-        if (t + 3 < T) v = *reinterpret_cast<const f4u*>(mass + t);
-        else v = f4{mass[min(t, T - 1)], mass[min(t + 1, T - 1)], mass[min(t + 2, T - 1)], mass[T - 1]};
+        if (t + 3 < end) v = *reinterpret_cast<const f4u*>(mass + t);
+        else v = f4{mass[min(t, end - 1)], mass[min(t + 1, end - 1)], mass[min(t + 2, end - 1)], mass[end - 1]};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) k[j] = t + j >= T ? 0u : t + j < lo || t + j >= hi ? kKeyStays : mass_key(v[j]);
-    };
-    if (N > 0) {                                                           // read by the thread that writes them
-#pragma unroll 4
-        for (int q = 0; q < Q; ++q) {
-            unsigned k[4];
-            load4((q * 64 * W + tid) * 4, k);
-            keys[q * 64 * W + tid] = uint4{k[0], k[1], k[2], k[3]};
-        }
+        for (int j = 0; j < 4; ++j) k[j] = t + j >= end ? 0u : t + j < lo || t + j >= hi ? kKeyStays : mass_key(v[j]);
     }
-    auto each = [&](int t0, auto f) {                                      // f(group, position, keys) over the sweep from t0
-#pragma unroll 4
-        for (int q = 0; q < Q; ++q) {
-            unsigned k[4];
-            const int t = t0 + (q * 64 * W + tid) * 4;
-            if (N > 0) { const uint4 v = keys[q * 64 * W + tid]; k[0] = v.x; k[1] = v.y; k[2] = v.z; k[3] = v.w; }
-            else load4(t, k);
-            f(q, t, k);
-        }
-    };
-    constexpr int SWEEP = Q * 256 * W;
-    int shift = 32;
-#pragma unroll 1
-    while (shift > 0) {
-        const int bits = shift < BITS ? shift : BITS, prev = shift;
-        const bool first = shift == 32;
-        shift -= bits;
-        const unsigned mask = (1u << bits) - 1;
-        for (int i = tid; i < B * R; i += 64 * W) hist[i] = 0;
-        __syncthreads();
-        for (int t0 = 0; t0 < T; t0 += SWEEP)
-            each(t0, [&](int, int, const unsigned (&k)[4]) {
+};
+// Of the keys that start with prefix, `same` of them, the `need` heaviest stay; the bits of all keys below prefix's are still open.
+struct Pick { unsigned prefix, need, same; };
+// The next `bits` of the threshold from the counts of their values, thread t holding those of mask - (t PT + i).  to: 3 words
+template <int W, int PT> __device__ __forceinline__ Pick pick_bits(const unsigned (&c)[PT], int bits, Pick p, unsigned* sm, unsigned* to) {
+    const unsigned mask = (1u << bits) - 1;
+    unsigned mine = 0, total;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (first || (k[j] >> prev) == prefix) atomicAdd(&hist[((k[j] >> shift) & mask) * R + lane % R], 1u);    // integers: the order changes nothing
-            });
-        __syncthreads();
-        unsigned c[PT], mine = 0, total;
+    for (int i = 0; i < PT; ++i) mine += c[i];
+    unsigned above = block_scan<W>(mine, sm, &total);
 #pragma unroll
-        for (int i = 0; i < PT; ++i) {
-            const int d = (int)mask - (tid * PT + i);
-            c[i] = 0;
-            if (d >= 0) { const uint2 v = *reinterpret_cast<const uint2*>(hist + d * R); c[i] = v.x + v.y; }
-            mine += c[i];
-        }
-        unsigned above = block_scan<W>(mine, sm, &total);
-#pragma unroll
-        for (int i = 0; i < PT; ++i) {
-            if (above < need && need <= above + c[i]) { pick[0] = mask - (unsigned)(tid * PT + i); pick[1] = need - above; pick[2] = c[i]; }
-            above += c[i];
-        }
-        __syncthreads();
-        prefix = bits == 32 ? pick[0] : (prefix << bits) | pick[0];
-        need = pick[1]; same = pick[2];
+    for (int i = 0; i < PT; ++i) {
+        if (above < p.need && p.need <= above + c[i]) { to[0] = mask - (threadIdx.x * PT + i); to[1] = p.need - above; to[2] = c[i]; }
+        above += c[i];
     }
+    __syncthreads();
+    return Pick{(p.prefix << bits) | to[0], to[1], to[2]};
+}
+// The kept positions of [t0, end) in order.  each(t0, f) calls f(group, position, keys) for this thread's groups of four from t0, Q at most and none that begins behind end; cnt: Q W words
+template <int W, int Q, typename Each>
+__device__ __forceinline__ void place_kept(int t0, int end, Pick p, unsigned ties_before, unsigned kept_before, const float* mass, int32_t* kept, float* mass_out, unsigned* sm,
+                                           unsigned* cnt, Each each) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, tid = threadIdx.x;
     // stays: heavier than the threshold, or equal to it and among the first `need` of those
-    const bool all_ties = need == same;                                    // then nobody's rank matters
-    unsigned ties_before = 0, kept_before = 0, all;
+    const bool all_ties = p.need == p.same;                                // then nobody's rank matters
+    const unsigned long long below = (1ull << lane) - 1;
+    unsigned all;
+    auto place = [&](const bool (&f)[4], int (&at)[4]) {                   // places of the set flags within the wave's 256 positions, and their number
+        unsigned long long b[4];
+        int n = 0, base = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { b[j] = __ballot(f[j]); n += (int)__popcll(b[j]); base += (int)__popcll(b[j] & below); }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { at[j] = base; base += f[j]; }
+        return n;
+    };
+    auto sum_up = [&](unsigned before, int groups) {                       // cnt -> what lies before each of its entries
+        __syncthreads();
+        static_assert(Q * W <= 64 * W, "one entry a thread");
+        const unsigned v = block_scan<W>(tid < groups * W ? cnt[tid] : 0u, sm, &all) + before;
+        if (tid < Q * W) cnt[tid] = v;
+        __syncthreads();
+    };
 #pragma unroll 1
-    for (int t0 = 0; t0 < T; t0 += SWEEP) {
-        const unsigned long long below = (1ull << lane) - 1;
-        auto place = [&](const bool (&f)[4], int (&at)[4]) {               // places of the set flags within the wave's 256 positions, and their number
-            unsigned long long b[4];
-            int n = 0, base = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { b[j] = __ballot(f[j]); n += (int)__popcll(b[j]); base += (int)__popcll(b[j] & below); }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { at[j] = base; base += f[j]; }
-            return n;
-        };
-        auto sum_up = [&](unsigned before) {                               // cnt -> what lies before each of its entries
-            __syncthreads();
-            static_assert(Q * W <= 64 * W, "one entry a thread");
-            const unsigned v = block_scan<W>(tid < Q * W ? cnt[tid] : 0u, sm, &all) + before;
-            if (tid < Q * W) cnt[tid] = v;
-            __syncthreads();
-        };
+    for (; t0 < end; t0 += Q * 256 * W) {
+        const int groups = min(Q, (end - t0 + 256 * W - 1) / (256 * W));   // those that `each` visits
         unsigned long long ties = 0;                                       // bit 4 q + j: equal to the threshold and among the first
         if (!all_ties) {
             each(t0, [&](int q, int, const unsigned (&k)[4]) {
                 bool f[4]; int at[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) f[j] = k[j] == prefix;
+                for (int j = 0; j < 4; ++j) f[j] = k[j] == p.prefix;
                 const int n = place(f, at);
                 if (lane == 0) cnt[q * W + w] = (unsigned)n;
             });
-            sum_up(ties_before);
+            sum_up(ties_before, groups);
             ties_before += all;
             each(t0, [&](int q, int, const unsigned (&k)[4]) {
                 bool f[4]; int at[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) f[j] = k[j] == prefix;
+                for (int j = 0; j < 4; ++j) f[j] = k[j] == p.prefix;
                 place(f, at);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) ties |= (unsigned long long)(f[j] && cnt[q * W + w] + (unsigned)at[j] < need) << (4 * q + j);
+                for (int j = 0; j < 4; ++j) ties |= (unsigned long long)(f[j] && cnt[q * W + w] + (unsigned)at[j] < p.need) << (4 * q + j);
             });
             __syncthreads();
         }
         auto stays = [&](int q, const unsigned (&k)[4], bool (&f)[4]) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = all_ties ? k[j] >= prefix : k[j] > prefix || (ties >> (4 * q + j) & 1);
+            for (int j = 0; j < 4; ++j) f[j] = all_ties ? k[j] >= p.prefix : k[j] > p.prefix || (ties >> (4 * q + j) & 1);
         };
         each(t0, [&](int q, int, const unsigned (&k)[4]) {
             bool f[4];
@@ -318,7 +281,7 @@ __global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, i
             for (int j = 0; j < 4; ++j) n += (int)__popcll(__ballot(f[j]));
             if (lane == 0) cnt[q * W + w] = (unsigned)n;
         });
-        sum_up(kept_before);
+        sum_up(kept_before, groups);
         kept_before += all;
         each(t0, [&](int q, int t, const unsigned (&k)[4]) {
             bool f[4]; int at[4];
@@ -328,12 +291,147 @@ __global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, i
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (f[j]) {
-                    kept[(size_t)h * n_keep + base + (unsigned)at[j]] = t + j;
-                    if (mass_out) mass_out[(size_t)h * ld_out + base + (unsigned)at[j]] = k[j] == kKeyStays ? mass[t + j] : key_mass(k[j]);
+                    kept[base + (unsigned)at[j]] = t + j;
+                    if (mass_out) mass_out[base + (unsigned)at[j]] = k[j] == kKeyStays ? mass[t + j] : key_mass(k[j]);
                 }
         });
         __syncthreads();
     }
+}
+// One workgroup per head.  With N > 0 (T <= 64 W N) a thread's N keys stay in LDS, else every pass reads the weights again, 64 a thread at a time.
+// (Registers would hold them too, but loops over them have to be unrolled, and then spill.)
+template <int W, int N, int BITS>
+__global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, int n_sink, int n_recent, const float* __restrict__ mass_in, int64_t ld_in,
+                                                            float* __restrict__ mass_out, int64_t ld_out, int32_t* __restrict__ kept) {
+    constexpr int Q = (N > 0 ? N : 64) / 4, R = 2, B = 1 << BITS, PT = (B + 64 * W - 1) / (64 * W);     // groups of four a thread and sweep; copies; buckets; buckets a thread
+    __shared__ unsigned hist[B * R], sm[W], to[3], cnt[Q * W];
+    extern __shared__ __align__(16) char smem[];
+    uint4* keys = reinterpret_cast<uint4*>(smem);                          // [Q][64 W]
+    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const Weights m{mass_in + (size_t)h * ld_in, n_sink, T - n_recent, T};
+    if (N > 0) {                                                           // read by the thread that writes them
+#pragma unroll 4
+        for (int q = 0; q < min(Q, (T + 256 * W - 1) / (256 * W)); ++q) {
+            unsigned k[4];
+            m.load4((q * 64 * W + tid) * 4, k);
+            keys[q * 64 * W + tid] = uint4{k[0], k[1], k[2], k[3]};
+        }
+    }
+    auto each = [&](int t0, auto f) {                                      // f(group, position, keys) over the sweep from t0
+        const int groups = min(Q, (T - t0 + 256 * W - 1) / (256 * W));     // nothing lies behind them
+        for (int q = 0; q < groups; ++q) {
+            unsigned k[4];
+            const int t = t0 + (q * 64 * W + tid) * 4;
+            if (N > 0) { const uint4 v = keys[q * 64 * W + tid]; k[0] = v.x; k[1] = v.y; k[2] = v.z; k[3] = v.w; }
+            else m.load4(t, k);
+            f(q, t, k);
+        }
+    };
+    Pick p{0, (unsigned)n_keep, 0};
+    int shift = 32;
+#pragma unroll 1
+    while (shift > 0) {
+        const int bits = shift < BITS ? shift : BITS, prev = shift;
+        const bool first = shift == 32;
+        shift -= bits;
+        const unsigned mask = (1u << bits) - 1;
+        for (int i = tid; i < B * R; i += 64 * W) hist[i] = 0;
+        __syncthreads();
+        for (int t0 = 0; t0 < T; t0 += Q * 256 * W)
+            each(t0, [&](int, int, const unsigned (&k)[4]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (k[j] != 0 && (first || (k[j] >> prev) == p.prefix)) atomicAdd(&hist[((k[j] >> shift) & mask) * R + lane % R], 1u);    // integers: the order changes nothing
+            });
+        __syncthreads();
+        unsigned c[PT];
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+            const int d = (int)mask - (tid * PT + i);
+            c[i] = 0;
+            if (d >= 0) { const uint2 v = *reinterpret_cast<const uint2*>(hist + d * R); c[i] = v.x + v.y; }
+        }
+        p = pick_bits<W, PT>(c, bits, p, sm, to);
+    }
+    place_kept<W, Q>(0, T, p, 0u, 0u, m.mass, kept + (size_t)h * n_keep, mass_out ? mass_out + (size_t)h * ld_out : nullptr, sm, cnt, each);
+}
+// Long sets on few heads: a head's positions are cut into gridDim.x slices, a workgroup each, and a launch for each of the threshold's three parts
+// (11, 11 and 10 bits) leaves the slices' counts for the next one, where every workgroup adds them up; the fourth places what stays.
+//   count  [3][heads][slices][2048]   of the part's values, heaviest first
+//   above  [2][heads][slices]         a slice's keys above the first (second) part of the threshold
+//   picks  [2][heads][4]              the threshold after the first (second) part
+struct Slices { unsigned *count, *above, *picks; };
+template <int PART>
+__global__ __launch_bounds__(1024) void kv8_select_slice_kernel(int T, int slice, int n_keep, int n_sink, int n_recent, const float* __restrict__ mass_in, int64_t ld_in,
+                                                                float* __restrict__ mass_out, int64_t ld_out, int32_t* __restrict__ kept, Slices s) {
+    constexpr int W = 16, Q = 2, R = 4;
+    constexpr int shift = PART == 0 ? 21 : PART == 1 ? 10 : 0, bits = PART < 2 ? 11 : 10, known = PART == 0 ? 0 : shift + bits, prev_bits = PART == 3 ? 10 : 11;
+    __shared__ unsigned hist[PART < 3 ? 2048 * R : 1], sm[W], to[3], tied, cnt[Q * W];
+    const int h = blockIdx.y, id = blockIdx.x, n = gridDim.x, tid = threadIdx.x, lane = tid & 63, heads = gridDim.y;
+    const int t0 = min(id * slice, T), end = min(t0 + slice, T);
+    const Weights m{mass_in + (size_t)h * ld_in, n_sink, T - n_recent, end};
+    auto each = [&](int t0, auto f) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            unsigned k[4];
+            const int t = t0 + (q * 64 * W + tid) * 4;
+            if (t0 + q * 256 * W >= end) break;
+            m.load4(t, k);
+            f(q, t, k);
+        }
+    };
+    Pick p{0, (unsigned)n_keep, 0};
+    unsigned kept_before = 0, ties_before = 0;
+    if (PART > 0) {                                                        // the previous part: thread t has its values 2 t and 2 t + 1, heaviest first
+        const uint2* c = reinterpret_cast<const uint2*>(s.count + ((size_t)(PART - 1) * heads + h) * n * 2048) + tid;
+        unsigned all[2] = {0, 0}, early[2] = {0, 0}, mine[2] = {0, 0};     // of all slices, of those before this one, of this one
+        for (int i = 0; i < n; ++i) {
+            const uint2 v = c[(size_t)i * 1024];
+            all[0] += v.x; all[1] += v.y;
+            if (i < id) { early[0] += v.x; early[1] += v.y; }
+            if (i == id) { mine[0] = v.x; mine[1] = v.y; }
+        }
+        if (PART > 1) { const unsigned* q = s.picks + ((size_t)(PART - 2) * heads + h) * 4; p = Pick{q[0], q[1], q[2]}; }
+        p = pick_bits<W, 2>(all, prev_bits, p, sm, to);
+        const unsigned at = ((1u << prev_bits) - 1) - (p.prefix & ((1u << prev_bits) - 1));    // the place of the threshold's value
+        auto heavier = [&](const unsigned (&v)[2]) { return (2u * tid < at ? v[0] : 0u) + (2u * tid + 1 < at ? v[1] : 0u); };
+        if (PART < 3) {
+            unsigned above;
+            (void)block_scan<W>(heavier(mine), sm, &above);
+            if (tid == 0) {
+                s.above[((size_t)(PART - 1) * heads + h) * n + id] = above;
+                if (id == 0) { unsigned* q = s.picks + ((size_t)(PART - 1) * heads + h) * 4; q[0] = p.prefix; q[1] = p.need; q[2] = p.same; }
+            }
+        } else {
+            unsigned x = heavier(early);
+            for (int i = tid; i < id; i += 1024) x += s.above[(size_t)h * n + i] + s.above[((size_t)heads + h) * n + i];
+            (void)block_scan<W>(x, sm, &kept_before);
+            if (2u * tid == (at & ~1u)) tied = early[at & 1];
+            __syncthreads();
+            ties_before = tied;
+            kept_before += min(ties_before, p.need);
+        }
+    }
+    if (PART < 3) {
+        for (int i = tid; i < 2048 * R / 4; i += 1024) reinterpret_cast<uint4*>(hist)[i] = uint4{0, 0, 0, 0};
+        __syncthreads();
+        for (int t = t0; t < end; t += Q * 256 * W)
+            each(t, [&](int, int t, const unsigned (&k)[4]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (t + j < end && (PART == 0 || (k[j] >> known) == p.prefix)) atomicAdd(&hist[((k[j] >> shift) & ((1u << bits) - 1)) * R + lane % R], 1u);
+            });
+        __syncthreads();
+        unsigned c[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int d = (1 << bits) - 1 - (2 * tid + i);
+            const uint4 v = reinterpret_cast<const uint4*>(hist)[max(d, 0)];
+            c[i] = d >= 0 ? v.x + v.y + v.z + v.w : 0u;
+        }
+        reinterpret_cast<uint2*>(s.count + (((size_t)PART * heads + h) * n + id) * 2048)[tid] = uint2{c[0], c[1]};
+    } else
+        place_kept<W, Q>(t0, end, p, ties_before, kept_before, m.mass, kept + (size_t)h * n_keep, mass_out ? mass_out + (size_t)h * ld_out : nullptr, sm, cnt, each);
 }
 // One workgroup per destination block, head and K | V: gathers the 16 kept rows as values and quantises them anew.  Sixteen rows that were
 // one block stay as they are (codes and scale), so that what eviction leaves in place does not drift.
@@ -1202,7 +1300,18 @@ hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_ou
     return hipGetLastError();
 }
 hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recent, const float* mass_in, int64_t ld_in, float* mass_out, int64_t ld_out, int32_t* kept,
-                             hipStream_t st) {
+                             unsigned* work, int64_t work_words, hipStream_t st) {
+    const int64_t slices = std::min((T + 4095) / 4096, (int)std::min<int64_t>(work_words / (Hkv * kKv8SliceWords), 64));
+    if (T > 32768 && slices >= 2) {
+        const int n = (int)slices, slice = ((T + n - 1) / n + 3) & ~3;
+        Slices s{work, work + (size_t)3 * Hkv * n * 2048, nullptr};
+        s.picks = s.above + (size_t)2 * Hkv * n;
+        auto part = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(n, Hkv), dim3(1024), 0, st, T, slice, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, ld_out, kept, s);
+        };
+        part(kv8_select_slice_kernel<0>); part(kv8_select_slice_kernel<1>); part(kv8_select_slice_kernel<2>); part(kv8_select_slice_kernel<3>);
+        return hipGetLastError();
+    }
 #define KV8_SELECT(W, N, BITS)                                                                                                                       \
     do {                                                                                                                                           \
         const size_t lds = (size_t)N * 64 * W * 4;                                                                                                 \
@@ -1211,6 +1320,8 @@ hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recen
         hipLaunchKernelGGL((kv8_select_kernel<W, N, BITS>), dim3(Hkv), dim3(64 * W), lds, st, T, n_keep, n_sink, n_recent, mass_in, ld_in, mass_out, \
                            ld_out, kept);                                                                                                          \
     } while (0)
+    // 32 heads, with the move of 64 positions (4 us): T = 5000 14 us, 32768 27; 8 heads, T = 65536 67 us on one workgroup a head, 37 in slices,
+    // 131072 125 and 44; in slices T = 32768 would take 30
     if (T <= 1024) KV8_SELECT(4, 4, 8);
     else if (T <= 4096) KV8_SELECT(16, 4, 11);
     else if (T <= 32768) KV8_SELECT(16, 32, 11);

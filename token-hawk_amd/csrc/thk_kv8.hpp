@@ -10,6 +10,7 @@ static const int kKv8Tile = 64;       // positions one step of the split attenti
 static const int kKv8Pad = 128;       // a cache holds whole multiples of this many positions: no kernel's step reads behind it
 static const int kKv8SplitRows = 8192; // rows x splits whose parts the workspace holds
 static const int kKv8Groups = 512;    // column groups x K/V heads up to which the positions are split (and counters there are)
+static const int kKv8SliceWords = 3 * 2048 + 16; // what the selection of long sets keeps for a slice of a head, in words
 static const int kKv8RowSlab = 2048;  // prompt rows one attention launch takes (sizes the per-row statistics)
 
 // Device memory of one cache.  n_blk = blocks per head, a multiple of 8 (kKv8Pad).
@@ -55,7 +56,7 @@ constexpr int kv8_split_waves(int D) { return D == 256 ? 4 : 8; }      // of a w
 hipError_t launch_kv8_append(const Kv8View& c, const float* k, const float* v, int64_t pos, int64_t n, hipStream_t st);
 hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_out, float* v_out, hipStream_t st);
 hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recent, const float* mass_in, int64_t ld_in, float* mass_out, int64_t ld_out, int32_t* kept,
-                             hipStream_t st);
+                             unsigned* work, int64_t work_words, hipStream_t st);
 hipError_t launch_kv8_move(const Kv8View& src, const Kv8View& dst, int n_keep, const int32_t* kept, hipStream_t st);
 hipError_t launch_kv8_attn_tile(const Kv8Attn& a, hipStream_t st);
 hipError_t launch_kv8_attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t st);
