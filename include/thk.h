@@ -366,6 +366,7 @@ int thk_peer_destroy(thk_peer* p);
  * The cache does not count positions: the caller passes them, as for thk_kv_append, and has appended [0, T) before it attends to T.  Calls are
  * stream-ordered, allocate nothing and may be captured into a graph (create and destroy may not); a replay uses the captured positions and
  * pointers.  The cache owns the workspace of its calls: calls and replays of ONE cache must not overlap on two streams.
+ * Outputs must not overlap inputs or each other, but for mass_in = mass_out in attention.
  * All pointers are 16-byte aligned dev pointers; weight arrays ("mass") are f32 [H_kv][n_ctx of their cache], only the entries named are touched. */
 typedef struct thk_kv8 thk_kv8;
 #define THK_KV8_BLOCK 16

@@ -389,6 +389,64 @@ def test_offsets_beyond_32_bits(thk, ctx):
     kv.close()
 
 
+@pytest.mark.parametrize("H,Hkv,D", [(64, 64, 64), (64, 64, 128), (128, 64, 64), (48, 48, 256)])
+@pytest.mark.parametrize("M", [129, 200, 300, 600, 700])
+def test_prefill_many_columns(thk, ctx, H, Hkv, D, M):
+    """Every shape of the many-rows kernel: one or two groups of waves, narrow and wide columns, columns that end inside one."""
+    rng = np.random.default_rng(M + H + D)
+    n_past = M % 97
+    T = n_past + M
+    p = Pair(thk, ctx, T + 1, H, Hkv, D)
+    p.append(rows(rng, T, Hkv, D), 0)
+    p.check(rng.standard_normal((M, H, D)).astype(np.float32), n_past, mass=rng.random((Hkv, T + 1)).astype(np.float32))
+
+
+def test_decode_of_many_heads(thk, ctx):
+    """More K/V heads than the positions are split for: a single row on the many-rows kernel."""
+    rng = np.random.default_rng(21)
+    p = Pair(thk, ctx, 131, 600, 600, 64)
+    p.append(rows(rng, 131, 600, 64), 0)
+    for T in (1, 64, 131):
+        p.check(rng.standard_normal((1, 600, 64)).astype(np.float32), T - 1, mass=np.zeros((600, 131), np.float32), decode=True)
+
+
+@pytest.mark.parametrize("T", [4095, 4096, 4097, 9001])
+@pytest.mark.parametrize("H,Hkv,D", [(2, 2, 64), (9, 3, 128), (16, 1, 128), (32, 2, 64), (17, 1, 64), (4, 2, 256)])
+def test_weights_of_longer_caches(thk, ctx, H, Hkv, D, T):
+    """Weights counted by the launch itself, by the joining launch and (groups of more than 16 heads) by one of their own."""
+    rng = np.random.default_rng(T + H)
+    p = Pair(thk, ctx, T + 3, H, Hkv, D)
+    p.append(rows(rng, T, Hkv, D), 0)
+    q = rng.standard_normal((1, H, D)).astype(np.float32)
+    p.check(q, T - 1, mass=rng.random((Hkv, T + 3)).astype(np.float32), decode=True)
+    p.check(q, T - 1, decode=True)
+
+
+@pytest.mark.parametrize("H,Hkv,D,pieces", [(16, 16, 128, 17), (64, 32, 64, 17), (8, 8, 256, 17), (32, 2, 128, 130)])
+def test_long_cache_past_the_caches(thk, ctx, H, Hkv, D, pieces):
+    """Codes of 64 MB and more: a piece of 1024 positions over and over, so that out is the piece's and each weight a share of the piece's."""
+    rng = np.random.default_rng(D + pieces)
+    n = 1024
+    T = n * pieces
+    x = rows(rng, n, Hkv, D)
+    ref = RefCache(n, Hkv, D)
+    ref.append(x[0], x[1], 0)
+    kv = thk.KvCache8(ctx, T, H, Hkv, D)
+    dk, dv = ctx.from_numpy(x[0]), ctx.from_numpy(x[1])
+    for at in range(0, T, n):
+        kv.append(dk, dv, at, n)
+    q = rng.standard_normal((1, H, D)).astype(np.float32)
+    dm, do = ctx.from_numpy(np.zeros((Hkv, T), np.float32)), ctx.alloc(q.nbytes)
+    kv.attn_decode(ctx.from_numpy(q), T, do, dm, dm)
+    eo, em, to, tm = attention(ref.values(), q, n - 1, np.zeros((Hkv, n), np.float32))
+    more = (T - n) / 16 * EPS                                       # the longer sums' share of the bounds
+    out, m = do.download(np.float32, q.shape), dm.download(np.float32, (Hkv, pieces, n))
+    assert np.all(np.abs(out - eo) <= to + 2 * more * np.abs(ref.values()[1]).max())
+    assert np.linalg.norm(out - eo) / np.linalg.norm(eo) < 1e-5
+    assert np.all(np.abs(m * pieces - em[:, None]) <= (tm + more * em)[:, None] + 1e-12)
+    kv.close()
+
+
 class Hip:
     """The HIP runtime the library runs on: streams and graphs for the tests."""
 
@@ -457,6 +515,54 @@ def test_captured_and_replayed(thk):
         hip.hipGraphDestroy(graph)
         kv.close()
         to.close()
+
+
+def test_captured_long_prompt_and_eviction(thk):
+    """The kernels that need more LDS than a launch gets unasked, and the selection in slices, first called inside a capture."""
+    rng = np.random.default_rng(22)
+    H, D, T, M, keep = 24, 64, 33000, 500, 700
+    with thk.Context(0) as c:
+        hip, st = Hip(), C.c_void_p(c.stream)
+        kv, a, b = thk.KvCache8(c, T, H, H, D), thk.KvCache8(c, keep, H, H, D), thk.KvCache8(c, keep, H, H, D)
+        x = rng.standard_normal((2, 1000, H, D), np.float32)
+        k, v = c.from_numpy(x[0]), c.from_numpy(x[1])
+        for at in range(0, T, 1000):
+            kv.append(k, v, at, 1000)
+        q, mass = c.from_numpy(rng.standard_normal((M, H, D)).astype(np.float32)), c.from_numpy(np.exp(rng.standard_normal((H, T)) * 2).astype(np.float32))
+        outs = [c.alloc(M * H * D * 4), c.alloc(H * T * 4)] + [c.alloc(H * keep * 4) for _ in range(4)]
+        om, m1, ka, ma, kb, mb = outs
+
+        def step():
+            kv.attn_prefill(q, 900, M, om, mass, m1)
+            kv.evict(a, T, keep, 4, 16, mass, ma, ka)
+            kv.evict(b, 20000, keep, 0, 0, mass, mb, kb)
+
+        c.sync()
+        graph, run = C.c_void_p(), C.c_void_p()
+        hip.hipStreamBeginCapture(st, 2)
+        try:
+            step()
+        finally:
+            hip.hipStreamEndCapture(st, C.byref(graph))
+        hip.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0))
+        for i in range(3):
+            q.upload(rng.standard_normal((M, H, D)).astype(np.float32))
+            mass.upload(np.exp(rng.standard_normal((H, T)) * 2).astype(np.float32))
+            for o in outs:
+                o.upload(np.zeros(o.nbytes // 4, np.float32))
+            hip.hipGraphLaunch(run, st)
+            c.sync()
+            got = [o.download(np.int32, o.nbytes // 4) for o in outs]
+            for o in outs:
+                o.upload(np.zeros(o.nbytes // 4, np.float32))
+            step()
+            c.sync()
+            for g, o in zip(got, outs):
+                assert np.array_equal(g, o.download(np.int32, o.nbytes // 4)), i
+        hip.hipGraphExecDestroy(run)
+        hip.hipGraphDestroy(graph)
+        for cache in (kv, a, b):
+            cache.close()
 
 
 def test_two_caches_on_two_streams(thk):

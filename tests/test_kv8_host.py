@@ -114,7 +114,12 @@ def test_refusals(env, lib, n_ctx):
                      (lambda: lib.thk_kv8_evict(kv, 30, 31, 0, 0, P, to, None, P), "n_keep=31"), (lambda: lib.thk_kv8_evict(kv, 100, 20, 10, 11, P, to, None, P), "exceed"),
                      (lambda: lib.thk_kv8_evict(kv, 100, 20, -1, 0, P, to, None, P), "exceed"), (lambda: lib.thk_kv8_evict(kv, 100, 20, big, big, P, to, None, P), "exceed"),
                      (lambda: lib.thk_kv8_evict(kv, 100, 20, 0, 0, None, to, None, P), "null"), (lambda: lib.thk_kv8_evict(kv, 100, 20, 0, 0, P, to, None, None), "null"),
-                     (lambda: lib.thk_kv8_evict(kv, 100, 20, 0, 0, P, to, P, P), "mass_out"), (lambda: lib.thk_kv8_evict(kv, 100, 20, 0, 0, P + 4, to, None, P), "aligned")]:
+                     (lambda: lib.thk_kv8_evict(kv, 100, 20, 0, 0, P, to, P, P), "mass_out"), (lambda: lib.thk_kv8_evict(kv, 100, 20, 0, 0, P, to, None, P + 1584), "overlap"),
+                     (lambda: lib.thk_kv8_evict(kv, 100, 20, 0, 0, P, to, P + 640, 3 * P), "overlap"), (lambda: lib.thk_kv8_evict(kv, 100, 20, 0, 0, P, to, 3 * P, 3 * P + 16), "overlap"),
+                     (lambda: lib.thk_kv8_read(kv, 0, 9, P, P + 9 * 1024 - 16), "overlap"), (lambda: lib.thk_kv8_attn_decode(kv, P, 5, None, None, P), "q and out"),
+                     (lambda: lib.thk_kv8_attn_prefill(kv, P, 0, 2, None, None, P + 2 * 2048 - 16), "q and out"), (lambda: lib.thk_kv8_attn_decode(kv, P, 5, 8 * P, 8 * P + 16, 4 * P), "not the same"),
+                     (lambda: lib.thk_kv8_attn_decode(kv, P, 5, 8 * P, 8 * P, 8 * P + 1200), "weights overlap"), (lambda: lib.thk_kv8_attn_decode(kv, P, 5, 8 * P, P + 16, 4 * P), "weights overlap"),
+                     (lambda: lib.thk_kv8_evict(kv, 100, 20, 0, 0, P + 4, to, None, P), "aligned")]:
         assert rc() == INVALID and text in env.err, (text, env.err)
     assert lib.stub_log() == b""                       # nothing was launched
     assert lib.thk_kv8_evict(kv, 100, 20, 0, 0, P, None, None, P) == INVALID
@@ -127,13 +132,13 @@ def test_launches_run_on_the_contexts_device_and_errors_come_back(lib):
     lib.stub_set(1, 0, 0, 0)
     kv, to = env.create(5000, 8, 4, 64), env.create(50, 8, 4, 64)
     lib.stub_log()
-    assert lib.thk_kv8_append(kv, P, P, 7, 20) == 0 and lib.thk_kv8_evict(kv, 100, 20, 4, 5, P, to, 2 * P, P) == 0
+    assert lib.thk_kv8_append(kv, P, P, 7, 20) == 0 and lib.thk_kv8_evict(kv, 100, 20, 4, 5, 64 * P, to, 2 * P, P) == 0
     assert lib.stub_log() == b"3:append 7 20;3:select 4 100 20 4 5 5000 50;3:move 20;" and lib.stub_device() == 1
     lib.stub_set(1, 1, 0, 0)                           # inside a capture: the calls themselves are allowed, freeing the cache is not
     assert lib.thk_kv8_append(kv, P, P, 0, 1) == 0 and lib.thk_kv8_destroy(kv) == STATE and "captured" in env.err
     lib.stub_set(1, 0, 0, 1)
-    for call in (lambda: lib.thk_kv8_append(kv, P, P, 0, 1), lambda: lib.thk_kv8_read(kv, 0, 1, P, None), lambda: lib.thk_kv8_attn_decode(kv, P, 1, None, None, P),
-                 lambda: lib.thk_kv8_attn_prefill(kv, P, 0, 2, P, P, P), lambda: lib.thk_kv8_evict(kv, 100, 20, 4, 5, P, to, None, P)):
+    for call in (lambda: lib.thk_kv8_append(kv, P, P, 0, 1), lambda: lib.thk_kv8_read(kv, 0, 1, P, None), lambda: lib.thk_kv8_attn_decode(kv, P, 1, None, None, 4 * P),
+                 lambda: lib.thk_kv8_attn_prefill(kv, P, 0, 2, 64 * P, 64 * P, 4 * P), lambda: lib.thk_kv8_evict(kv, 100, 20, 4, 5, 64 * P, to, None, P)):
         assert call() == HIP and lib.stub_device() == 1
     lib.stub_set(1, 0, 0, 0)
     assert lib.thk_kv8_destroy(kv) == 0 and lib.thk_kv8_destroy(to) == 0 and lib.stub_device() == 1

@@ -13,7 +13,7 @@ struct thk_kv8 {
     float* part_o = nullptr;    // parts of rows that are split over the positions
     float2* part_ml = nullptr;
     unsigned* counters = nullptr;
-    float* scores = nullptr;    // [H][padded n_ctx]: a single row's scores, for the weight count
+    float* scores = nullptr;    // [H][padded n_ctx]: a single row's scores, for the weight count (groups of up to kKv8ScoredHeads heads)
 };
 
 namespace {
@@ -27,6 +27,7 @@ struct DeviceScope {
     }
     ~DeviceScope() { if (old >= 0) (void)hipSetDevice(old); }
 };
+bool overlap(const void* a, size_t na, const void* b, size_t nb) { return a && b && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -57,7 +58,7 @@ extern "C" int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_
     v.H = (int)H; v.Hkv = (int)H_kv; v.D = (int)D;
     const size_t codes = (size_t)H_kv * v.n_blk * kKv8Block * D, scales = up256((size_t)H_kv * v.n_blk * 4), tail = (size_t)2 * H_kv * kKv8Block * D * 4;
     const size_t at = up256((size_t)2 * H_kv * sizeof(int2)), ml = (size_t)kKv8RowSlab * H * sizeof(float2);
-    const size_t part = (size_t)kKv8SplitRows * (D * 4 + sizeof(float2)), scores_bytes = (size_t)H * v.n_blk * kKv8Block * 4;
+    const size_t part = (size_t)kKv8SplitRows * (D * 4 + sizeof(float2)), scores_bytes = H / H_kv <= kKv8ScoredHeads ? (size_t)H * v.n_blk * kKv8Block * 4 : 0;
     kv->mem_bytes = 2 * codes + 2 * scales + tail + at + ml + part + kKv8Groups * 4 + scores_bytes;
     hipError_t e = hipMalloc(&kv->mem, kv->mem_bytes);
     if (e != hipSuccess) {
@@ -120,6 +121,8 @@ extern "C" int thk_kv8_read(thk_kv8* kv, int64_t pos, int64_t n_tok, float* k_ou
     REQUIRE(ctx, pos <= kv->n_ctx && n_tok <= kv->n_ctx - pos, "thk_kv8_read: positions [%lld, %lld + %lld) outside the cache of %lld", (long long)pos, (long long)pos,
             (long long)n_tok, (long long)kv->n_ctx);
     REQUIRE(ctx, aligned16(k_out) && aligned16(v_out), "thk_kv8_read: k_out and v_out must be 16-byte aligned");
+    const size_t bytes = (size_t)n_tok * kv->view.Hkv * kv->view.D * 4;
+    REQUIRE(ctx, !overlap(k_out, bytes, v_out, bytes), "thk_kv8_read: k_out and v_out overlap");
     DeviceScope dev(ctx->device);
     HIPCHK(ctx, dev.err);
     HIPCHK(ctx, launch_kv8_read(kv->view, pos, n_tok, k_out, v_out, ctx->stream));
@@ -132,9 +135,13 @@ static int kv8_attention(thk_kv8* kv, const char* what, const float* q, int64_t 
     REQUIRE(ctx, q && out, "%s: null pointer", what);
     REQUIRE(ctx, (mass_in != nullptr) == (mass_out != nullptr), "%s: mass_in and mass_out go together", what);
     REQUIRE(ctx, aligned16(q) && aligned16(out) && aligned16(mass_in) && aligned16(mass_out), "%s: pointers must be 16-byte aligned", what);
+    const size_t row = (size_t)kv->view.H * kv->view.D, rows = (size_t)M * row * 4;
+    const size_t weights = ((size_t)(kv->view.Hkv - 1) * kv->n_ctx + n_past + M) * 4;                  // up to the last entry that is touched
+    REQUIRE(ctx, !overlap(q, rows, out, rows), "%s: q and out overlap", what);
+    REQUIRE(ctx, mass_in == mass_out || !overlap(mass_in, weights, mass_out, weights), "%s: mass_in and mass_out overlap and are not the same array", what);
+    REQUIRE(ctx, !overlap(out, rows, mass_in, weights) && !overlap(out, rows, mass_out, weights) && !overlap(q, rows, mass_out, weights), "%s: the weights overlap q or out", what);
     DeviceScope dev(ctx->device);
     HIPCHK(ctx, dev.err);
-    const size_t row = (size_t)kv->view.H * kv->view.D;
     for (int64_t i = 0; i < M; i += kKv8RowSlab) {
         Kv8Attn a{};
         a.c = kv->view; a.q = q + i * row; a.out = out + i * row;
@@ -142,8 +149,8 @@ static int kv8_attention(thk_kv8* kv, const char* what, const float* q, int64_t 
         if (mass_out) { a.ml = kv->ml; a.mass_in = mass_in; a.mass_out = mass_out; a.mass_ld = kv->n_ctx; a.mass_n = (int)(n_past + M); }
         bool scored = false;
         const int64_t G = a.c.H / a.c.Hkv, cols = a.M * G, cg = (cols + 15) / 16, groups = cg * a.c.Hkv;      // workgroups without a split
-        // Few columns: split over the positions, a tile of 64 a wave in turn; many: whole rows, tiles shared by a workgroup.  At 512 positions x 1024
-        // groups 29 | 18 us, at 8192 x 512 groups 100 | 190, x 1024 groups 185 | 196 (split | rows): the border is at 512 groups.
+        // Few columns: split over the positions, a tile of 64 a wave in turn; many: whole rows, tiles shared by a workgroup.  32 heads of 128, split and
+        // rows: no past, 512 groups 11.2 and 10.7 us, 768 17.6 and 12.9; over 1024 positions 22.6 and 29.3, 34.2 and 32.3; over 8192 91 and 148, 138 and 155.
         if (groups <= kKv8Groups) {
             Kv8Split sp{};
             const int64_t T = a.n_past + a.M, tiles = (T + kKv8Tile - 1) / kKv8Tile, waves = kv8_split_waves(a.c.D);
@@ -153,7 +160,7 @@ static int kv8_attention(thk_kv8* kv, const char* what, const float* q, int64_t 
             sp.stream = cg == 1 && 2 * T * a.c.Hkv * a.c.D >= (64 << 20);  // twice what the L2s hold: 112 -> 100 us at 65535 x 32 heads; at 2047 x 40 heads 10.4 -> 11.1
             // Joined inside the launch where the last workgroup has little to do: 4096 positions, 32 heads on 8, 10.4 -> 9.7 us, at 8192 10.8 -> 11.3; and
             // the weights counted there, too: 2048 positions 17.4 -> 13.2 us, 8192 19.6 -> 23.3.
-            const bool inside = sp.n * std::min<int64_t>(cols, 16) <= 64, count = mass_out && a.M == 1 && G <= 16;
+            const bool inside = sp.n * std::min<int64_t>(cols, 16) <= 64, count = mass_out && a.M == 1 && G <= kKv8ScoredHeads;
             const bool count_inside = inside && T <= 4096;
             scored = count && (count_inside || sp.n > 1);
             if (scored) { sp.scores = kv->scores; sp.scores_ld = (int64_t)a.c.n_blk * kKv8Block; }
@@ -189,6 +196,8 @@ extern "C" int thk_kv8_evict(thk_kv8* src, int64_t T, int64_t n_keep, int64_t n_
     REQUIRE(ctx, mass_in && kept, "thk_kv8_evict: null pointer");
     REQUIRE(ctx, mass_in != mass_out, "thk_kv8_evict: mass_out must not be mass_in");
     REQUIRE(ctx, aligned16(mass_in) && aligned16(mass_out) && aligned16(kept), "thk_kv8_evict: pointers must be 16-byte aligned");
+    const size_t in = ((size_t)(src->view.Hkv - 1) * src->n_ctx + T) * 4, to = ((size_t)(src->view.Hkv - 1) * dst->n_ctx + n_keep) * 4, list = (size_t)src->view.Hkv * n_keep * 4;
+    REQUIRE(ctx, !overlap(mass_in, in, mass_out, to) && !overlap(mass_in, in, kept, list) && !overlap(mass_out, to, kept, list), "thk_kv8_evict: mass_in, mass_out and kept overlap");
     DeviceScope dev(ctx->device);
     HIPCHK(ctx, dev.err);
     HIPCHK(ctx, launch_kv8_select(src->view.Hkv, (int)T, (int)n_keep, (int)n_sink, (int)n_recent, mass_in, src->n_ctx, mass_out, dst->n_ctx, kept,

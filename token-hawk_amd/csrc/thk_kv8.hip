@@ -60,6 +60,8 @@ template <int D> __device__ __forceinline__ void put_codes(int8_t* p, const unsi
 // their codes), the new ones from x [n][Hkv][D], and writes the whole block anew.  Because the open block is always requantised from
 // unrounded rows, n calls of one token leave the same bits as one call of n.  The last block's rows go to tail; when the call spans
 // several blocks the first workgroup also takes the last block, after the first: nobody else reads or writes tail.
+// Bound by memory: 16381 tokens on 32 heads of 128, 537 MB in and 134 MB out, 140 us, the rate of a large copy (4.8 TB/s).  A single token: the
+// launch (3.5 us); all its sources are asked for before one is chosen, so that it waits for memory once.
 template <int D, bool V>
 __device__ void append_block(const Kv8View& c, int h, int b, const float* x, int64_t pos, int64_t n, bool last, unsigned* sm) {
     const int64_t p0 = (int64_t)b * kKv8Block;
@@ -132,6 +134,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8View c, const float*
 }
 
 // ---------------------------------------------------------------- read
+// value = code * scale, a block per workgroup as for append.  Bound by the f32 stores: 16386 positions on 32 heads 152 us (4.4 TB/s).
 template <int D, bool V>
 __device__ __forceinline__ void read_body(const Kv8View& c, int64_t pos, int64_t n, float* out) {
     const int h = blockIdx.y, b = (int)(pos / kKv8Block) + blockIdx.x;
@@ -434,7 +437,8 @@ __global__ __launch_bounds__(1024) void kv8_select_slice_kernel(int T, int slice
         place_kept<W, Q>(t0, end, p, ties_before, kept_before, m.mass, kept + (size_t)h * n_keep, mass_out ? mass_out + (size_t)h * ld_out : nullptr, sm, cnt, each);
 }
 // One workgroup per destination block, head and K | V: gathers the 16 kept rows as values and quantises them anew.  Sixteen rows that were
-// one block stay as they are (codes and scale), so that what eviction leaves in place does not drift.
+// one block stay as they are (codes and scale), so that what eviction leaves in place does not drift.  A V row is a byte of every 16 (the layout
+// attention wants), so sparse selections read all of V: 4099 of 32768 positions on 32 heads, 134 MB of V and 51 MB else, 47 us.
 template <int D, bool V>
 __device__ __forceinline__ void move_body(const Kv8View& s, const Kv8View& d, int n_keep, const int32_t* kept, unsigned* sm, int* src) {
     const int h = blockIdx.y, b = blockIdx.x, rows = n_keep - b * kKv8Block < kKv8Block ? n_keep - b * kKv8Block : kKv8Block;
@@ -505,6 +509,9 @@ static const float kLog2e = 1.44269504088896340736f;      // scores carry log2(e
 // rows 4 (lane / 16) + i).  The k order is free as long as A and B share it, and the row order of the first product is chosen so that
 // lane chunk c ends up with the scores of the 16 positions of block c: then one K scale and one V scale per lane serve a whole tile, and
 // the second product's B operand is what the lane already holds - no exchange between lanes.
+// Long caches are bound by memory: 65535 positions on 32 heads, 537 MB in 89 us (6.0 TB/s; the bare reads in this pattern reach 6.9), 131071 on 8
+// heads for 64 query heads 47 us with the joining launch.  Short ones are a chain of latencies (launch, load, one or two tiles, join of the waves,
+// join of the splits): 64 positions 4.2 us, 512 on 32 heads with weights 8.0 us, 2047 on 40 heads 9.4 us.
 typedef int i4 __attribute__((ext_vector_type(4)));
 struct U2 { unsigned a, b; };
 // Between them, a and b hold a value and that of the lane 16 (32) away, in every lane.  The swap works on two registers: the empty asm keeps
@@ -549,13 +556,14 @@ __device__ __forceinline__ void pack_digits(unsigned e0, unsigned e1, unsigned e
 }
 __device__ __forceinline__ float join_digits(int i2, int i1, int i0) { return fmaf((float)i2, 65536.f, (float)(i1 * 256 + i0)); }   // |i1| <= 256 * 2^14: no overflow
 
-// The B operand of q: digits of columns n = 16 cg + lane % 16, dimensions 64 kc + 16 (lane / 16) + j.  Returns the step of the fixed point.
+// q of a column as a B operand wants it: x[4 kc + i] are dimensions 64 kc + 16 (lane / 16) + 4 i + 0 .. 3 (q points to the chunk's first)
 template <int D>
 __device__ __forceinline__ void load_q(const float* q, bool valid, f4 (&x)[D / 16]) {
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) x[i] = valid ? reinterpret_cast<const f4*>(q)[(i / 4) * 16 + i % 4] : f4{0.f, 0.f, 0.f, 0.f};
 }
-// digits of 4 N numbers of a lane as fixed point relative to the largest of their column, as put(word, d2, d1, d0); returns its step
+// Digits of 4 N numbers of a lane as fixed point relative to the largest of their column, as put(word, d2, d1, d0); returns its step.  One fma makes a
+// digit triple: 22 bits and the sign, half a step is 2^-23 of the largest entry (a step more cost three instructions each, 9 % of the weight count).
 template <int N, typename Max, typename Put>
 __device__ __forceinline__ float digits_of(const f4 (&x)[N], Max column_max, Put put) {
     unsigned m = 0;
@@ -853,7 +861,8 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_attn_split_kerne
 }
 // After a split that was not joined inside its launch.  The first M H workgroups join a row and head each: 256 / (D / 4) groups of threads take
 // the splits in turn.  The others (one row, scores left behind) count the weights: 512 positions of a K/V head each, with maxima and sums of
-// the group's heads from their parts, so that they need not wait for the join.
+// the group's heads from their parts, so that they need not wait for the join.  8 MB of scores and 8 MB of weights twice (65535 positions, 32
+// heads): 9 us.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_attn_finish_kernel(Kv8Attn a, Kv8Split sp) {
     constexpr int R = 256 / (D / 4);
@@ -929,6 +938,9 @@ __global__ __launch_bounds__(256) void kv8_attn_finish_kernel(Kv8Attn a, Kv8Spli
 //   weights p * v_scale in units of 2^(ref - 15), ref >= the exponent of the largest weight the column has met (relative to its running
 //           maximum): at most 2^15, and what the lo part cannot hold is below 2^-40 of that largest weight.  The accumulators are rescaled
 //           only where the running maximum or ref moves, which a wave skips when none of its columns did.
+// Bound by the matrix instructions and, beside them, the softmax's vector ones (on f16 the two do not overlap): 2048 rows over 6144 positions, 32
+// heads on 8, 420 us, 481 GFLOP of f16 products (the f32 work twice) at 1.15 PFLOP/s; a large f16 matrix product reaches 1.16.
+// S = 2: a second group of four waves takes every other tile, and its sums join the first's through LDS: 512 rows on 32 heads 18.8 -> 16.2 us.
 typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
 struct HF8x2 { hf8 a, b; };
@@ -1196,7 +1208,8 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
 // ---------------------------------------------------------------- weight count of many rows
 // mass_out = mass_in + sum over the columns of exp2(s - m) / l.  A workgroup takes 64 positions; its W waves share the columns, 16 at a time
 // in turn, each with the K fragments of all 64 positions in registers and the next columns' q on the way; the waves' sums are added in a
-// fixed order.
+// fixed order.  Scores anew instead of kept ones: [rows][heads][positions] would be hundreds of times the cache.  Bound by vector instructions (a
+// column's digits, 16 exponentials a lane): 512 rows on 32 heads 15 us, of which the first tile's workgroup, all rows' columns, is the longest.
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_mass_tile_kernel(Kv8Attn a, float scale) {
     constexpr int KC = D / 64;
@@ -1343,12 +1356,14 @@ template <int D, int NC, int S> static hipError_t attn_tile(const Kv8Attn& a, hi
     return hipGetLastError();
 }
 template <int D> static hipError_t attn_tile(const Kv8Attn& a, hipStream_t st) {
-    // 32 columns a wave halve the LDS reads of 16, once there are enough workgroups for every CU to hold two; where there is at most one workgroup
-    // a CU, a second group of waves takes every other tile.
-    const int64_t cols = (int64_t)a.M * (a.c.H / a.c.Hkv);
-    if ((cols + 127) / 128 * a.c.Hkv >= 384) return attn_tile<D, 2, 1>(a, st);
-    if ((cols + 63) / 64 * a.c.Hkv <= 256) return attn_tile<D, 1, 2>(a, st);
-    return attn_tile<D, 1, 1>(a, st);
+    // Wide: 32 columns a wave halve the LDS reads of 16.  Two groups of waves (S = 2) where there is at most one workgroup a CU: 512 rows on 32 heads
+    // 18.8 -> 16.2 us narrow, 1024 rows over 8192 positions 316 -> 273 us wide instead of narrow.  With more, one group, and two workgroups a CU;
+    // narrow ones until there are enough wide ones to share the CUs evenly: 800 rows on 40 heads (280 wide ones) 30 us narrow, 38 wide; 1500 rows
+    // over 8192 positions, 32 heads on 8 (376) 495 and 472, but from the start 52 and 67.
+    const int64_t cols = (int64_t)a.M * (a.c.H / a.c.Hkv), narrow = (cols + 63) / 64 * a.c.Hkv, wide = (cols + 127) / 128 * a.c.Hkv;
+    if (narrow <= 256) return attn_tile<D, 1, 2>(a, st);
+    if (wide <= 256) return attn_tile<D, 2, 2>(a, st);
+    return wide < 384 ? attn_tile<D, 1, 1>(a, st) : attn_tile<D, 2, 1>(a, st);
 }
 hipError_t launch_kv8_attn_tile(const Kv8Attn& a, hipStream_t st) {
     switch (a.c.D) {

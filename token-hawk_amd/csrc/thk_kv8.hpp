@@ -11,6 +11,7 @@ static const int kKv8Pad = 128;       // a cache holds whole multiples of this m
 static const int kKv8SplitRows = 8192; // rows x splits whose parts the workspace holds
 static const int kKv8Groups = 512;    // column groups x K/V heads up to which the positions are split (and counters there are)
 static const int kKv8SliceWords = 3 * 2048 + 16; // what the selection of long sets keeps for a slice of a head, in words
+static const int kKv8ScoredHeads = 16; // query heads of a K/V head up to which a single row's scores are kept for the weight count (else they are computed again)
 static const int kKv8RowSlab = 2048;  // prompt rows one attention launch takes (sizes the per-row statistics)
 
 // Device memory of one cache.  n_blk = blocks per head, a multiple of 8 (kKv8Pad).
