@@ -298,20 +298,22 @@ def test_evict(thk, ctx, Hkv, D, T, keep, sink, recent):
     assert np.array_equal(dst.read(0, keep + 5), dst.ref.values(0, keep + 5))
 
 
-@pytest.mark.parametrize("T,keep,Hkv", [(32768, 9000, 2), (32769, 20011, 2), (70001, 5, 2), (140000, 139999, 2), (33001, 4500, 44), (50002, 1234, 30), (1 << 20, 70000, 1)])
-def test_evict_long(thk, ctx, T, keep, Hkv):
+@pytest.mark.parametrize("T,keep,Hkv", [(32768, 9000, 2), (32769, 20011, 2), (70001, 5, 2), (140000, 139999, 2), (33001, 4500, 44), (50002, 1234, 30), (1 << 20, 70000, 1), (40001, 3, 2), (32001, 3, 2), (33333, 33333, 2)])
+@pytest.mark.parametrize("sink,recent", [(1, 2), (0, 0), (700, 20000)])
+def test_evict_long(thk, ctx, T, keep, Hkv, sink, recent):
     """The selection's other ranges: positions and weights only (the values of a few kept rows)."""
+    sink, recent = min(sink, keep // 2), min(recent, keep - min(sink, keep // 2))
     rng = np.random.default_rng(T)
     kv, dst = thk.KvCache8(ctx, T, Hkv, Hkv, 64), thk.KvCache8(ctx, keep, Hkv, Hkv, 64)
     mass = np.exp(rng.standard_normal((Hkv, T)) * 3).astype(np.float32)
     mass[Hkv // 2:] = np.round(mass[Hkv // 2:])                                     # ties by the thousand
     dm, mo, kept = ctx.from_numpy(mass), ctx.alloc(Hkv * keep * 4), ctx.alloc(Hkv * keep * 4)
-    kv.evict(dst, T, keep, 1, 2, dm, mo, kept)
+    kv.evict(dst, T, keep, sink, recent, dm, mo, kept)
     got, gm = kept.download(np.int32, (Hkv, keep)), mo.download(np.float32, (Hkv, keep))
     for h in range(Hkv):
-        mid = np.arange(1, T - 2)
-        heavy = mid[np.argsort(-mass[h, 1:T - 2].astype(np.float64), kind="stable")][:keep - 3]
-        exp = np.sort(np.concatenate([[0], heavy, [T - 2, T - 1]]))
+        mid = np.arange(sink, T - recent)
+        heavy = mid[np.argsort(-mass[h, sink:T - recent].astype(np.float64), kind="stable")][:keep - sink - recent]
+        exp = np.concatenate([np.arange(sink), np.sort(heavy), np.arange(T - recent, T)])
         assert np.array_equal(got[h], exp)
         assert np.array_equal(gm[h], mass[h][exp])
     kv.close()

@@ -208,6 +208,7 @@ struct Weights {                                                           // of
 };
 // Of the keys that start with prefix, `same` of them, the `need` heaviest stay; the bits of all keys below prefix's are still open.
 struct Pick { unsigned prefix, need, same; };
+static const Pick kOnlyThose = {kKeyStays, 1u, 1u};                        // nothing but what stays in any case
 // The next `bits` of the threshold from the counts of their values, thread t holding those of mask - (t PT + i).  to: 3 words
 template <int W, int PT> __device__ __forceinline__ Pick pick_bits(const unsigned (&c)[PT], int bits, Pick p, unsigned* sm, unsigned* to) {
     const unsigned mask = (1u << bits) - 1;
@@ -331,8 +332,9 @@ __global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, i
             f(q, t, k);
         }
     };
-    Pick p{0, (unsigned)n_keep, 0};
+    Pick p{0, (unsigned)(n_keep - n_sink - n_recent), 0};                  // what stays in any case is not counted
     int shift = 32;
+    if (p.need == 0) { p = kOnlyThose; shift = 0; }
 #pragma unroll 1
     while (shift > 0) {
         const int bits = shift < BITS ? shift : BITS, prev = shift;
@@ -345,7 +347,7 @@ __global__ __launch_bounds__(64 * W) void kv8_select_kernel(int T, int n_keep, i
             each(t0, [&](int, int, const unsigned (&k)[4]) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (k[j] != 0 && (first || (k[j] >> prev) == p.prefix)) atomicAdd(&hist[((k[j] >> shift) & mask) * R + lane % R], 1u);    // integers: the order changes nothing
+                    if (k[j] - 1 < kKeyStays - 1 && (first || (k[j] >> prev) == p.prefix)) atomicAdd(&hist[((k[j] >> shift) & mask) * R + lane % R], 1u);    // integers: the order changes nothing
             });
         __syncthreads();
         unsigned c[PT];
@@ -384,9 +386,13 @@ __global__ __launch_bounds__(1024) void kv8_select_slice_kernel(int T, int slice
             f(q, t, k);
         }
     };
-    Pick p{0, (unsigned)n_keep, 0};
+    Pick p{0, (unsigned)(n_keep - n_sink - n_recent), 0};
     unsigned kept_before = 0, ties_before = 0;
-    if (PART > 0) {                                                        // the previous part: thread t has its values 2 t and 2 t + 1, heaviest first
+    const bool only_those = p.need == 0;
+    if (only_those) {
+        if (PART < 3) return;
+        p = kOnlyThose;
+    } else if (PART > 0) {                                                        // the previous part: thread t has its values 2 t and 2 t + 1, heaviest first
         const uint2* c = reinterpret_cast<const uint2*>(s.count + ((size_t)(PART - 1) * heads + h) * n * 2048) + tid;
         unsigned all[2] = {0, 0}, early[2] = {0, 0}, mine[2] = {0, 0};     // of all slices, of those before this one, of this one
         for (int i = 0; i < n; ++i) {
@@ -416,6 +422,7 @@ __global__ __launch_bounds__(1024) void kv8_select_slice_kernel(int T, int slice
             kept_before += min(ties_before, p.need);
         }
     }
+    kept_before += (unsigned)(min(t0, m.lo) + max(t0 - m.hi, 0));          // stay in any case, before this slice
     if (PART < 3) {
         for (int i = tid; i < 2048 * R / 4; i += 1024) reinterpret_cast<uint4*>(hist)[i] = uint4{0, 0, 0, 0};
         __syncthreads();
@@ -423,7 +430,7 @@ __global__ __launch_bounds__(1024) void kv8_select_slice_kernel(int T, int slice
             each(t, [&](int, int t, const unsigned (&k)[4]) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (t + j < end && (PART == 0 || (k[j] >> known) == p.prefix)) atomicAdd(&hist[((k[j] >> shift) & ((1u << bits) - 1)) * R + lane % R], 1u);
+                    if (k[j] - 1 < kKeyStays - 1 && (PART == 0 || (k[j] >> known) == p.prefix)) atomicAdd(&hist[((k[j] >> shift) & ((1u << bits) - 1)) * R + lane % R], 1u);
             });
         __syncthreads();
         unsigned c[2];
