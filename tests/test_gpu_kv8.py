@@ -412,6 +412,16 @@ def test_decode_of_many_heads(thk, ctx):
         p.check(rng.standard_normal((1, 600, 64)).astype(np.float32), T - 1, mass=np.zeros((600, 131), np.float32), decode=True)
 
 
+@pytest.mark.parametrize("H,Hkv,T", [(260, 260, 4100), (400, 400, 130), (1024, 1, 700), (1024, 512, 65)])
+def test_decode_without_a_split(thk, ctx, H, Hkv, T):
+    """Column groups enough to fill the chip, or nearly: one part, weights counted in the launch (to 4096 positions) or by one of their own."""
+    rng = np.random.default_rng(H + T)
+    p = Pair(thk, ctx, T, H, Hkv, 64)
+    p.append(rows(rng, T, Hkv, 64), 0)
+    p.check(rng.standard_normal((1, H, 64)).astype(np.float32), T - 1, mass=rng.random((Hkv, T)).astype(np.float32), decode=True)
+    p.check(rng.standard_normal((3, H, 64)).astype(np.float32), T - 3, mass=rng.random((Hkv, T)).astype(np.float32))
+
+
 @pytest.mark.parametrize("T", [4095, 4096, 4097, 9001])
 @pytest.mark.parametrize("H,Hkv,D", [(2, 2, 64), (9, 3, 128), (16, 1, 128), (32, 2, 64), (17, 1, 64), (4, 2, 256)])
 def test_weights_of_longer_caches(thk, ctx, H, Hkv, D, T):
