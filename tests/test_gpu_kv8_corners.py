@@ -1,0 +1,47 @@
+"""The 8-bit K/V cache where its kernels' ranges end, beginning with every number of parts a long axis is cut into.  Plain form and bounds:
+tests/kv8_ref.py; caches and their plain twins: test_gpu_kv8.py."""
+import numpy as np
+import pytest
+
+from kv8_ref import attention
+from test_gpu_kv8 import Pair, rows
+
+pytestmark = pytest.mark.gpu
+
+
+def towards(rng, x, q, lo, gap):
+    """Keys [lo, end) of every K/V head get scores about `gap` above the others' for the head's first query."""
+    G, D = q.shape[0] // x.shape[2], q.shape[1]
+    for j in range(x.shape[2]):
+        u = q[j * G]
+        x[0, lo:, j] += u * (gap * np.sqrt(D) / (u @ u))
+
+
+@pytest.mark.parametrize("H,Hkv,D,step", [(6, 1, 64, 512), (4, 1, 128, 512), (4, 1, 256, 256)])
+def test_every_number_of_parts(thk, ctx, H, Hkv, D, step):
+    """A single row over 2 .. 64 parts (a part per `step` positions), joined in the launch or by one of its own, distinct values everywhere."""
+    rng = np.random.default_rng(D)
+    p = Pair(thk, ctx, 64 * step, H, Hkv, D)
+    p.append(rows(rng, 64 * step, Hkv, D), 0)
+    val, ld = p.ref.values(), 64 * step
+    for parts in range(2, 65):
+        T = parts * step - int(rng.integers(0, step - 64))
+        q = rng.standard_normal((1, H, D)).astype(np.float32)
+        mass = rng.random((Hkv, ld)).astype(np.float32)
+        eo, em, to, tm = attention(val[:, :T], q, T - 1, mass)
+        for m in (None, mass):
+            out, got = p.attend(q, T - 1, m, decode=True)
+            assert np.all(np.abs(out - eo) <= to), (parts, T, float((np.abs(out - eo) / to).max()))
+        assert np.all(np.abs(got[:, :T] - em) <= tm), (parts, T)
+
+
+@pytest.mark.parametrize("H,Hkv,D,T,M", [(16, 1, 64, 8500, 1), (30, 15, 64, 9001, 1), (32, 4, 128, 16500, 1), (16, 2, 128, 20500, 1), (8, 8, 64, 8600, 5), (16, 1, 64, 10300, 3), (4, 2, 128, 16700, 19)])
+def test_newest_positions_of_a_long_cache(thk, ctx, H, Hkv, D, T, M):
+    """The last part holds a large share of the weight: odd numbers of parts, single rows and a few rows."""
+    rng = np.random.default_rng(T)
+    p = Pair(thk, ctx, T + 3, H, Hkv, D)
+    x, q = rows(rng, T, Hkv, D), rng.standard_normal((M, H, D)).astype(np.float32)
+    towards(rng, x, q[M - 1], T - 40, 6)
+    p.append(x, 0)
+    p.check(q, T - M, decode=M == 1)
+    p.check(q, T - M, mass=rng.random((Hkv, T + 3)).astype(np.float32), decode=M == 1)

@@ -889,8 +889,10 @@ __global__ __launch_bounds__(256) void kv8_attn_finish_kernel(Kv8Attn a, Kv8Spli
         float e;
         const float2 ml = stats(r, e);
         f4 sum = f4{0.f, 0.f, 0.f, 0.f};
-        for (int i = g; i < sp.n; i += R) {
-            const float ei = __shfl(e, i);
+        for (int i0 = 0; i0 < sp.n; i0 += R) {                           // all lanes in every round: a lane that has left can give nobody its share
+            const int i = i0 + g;
+            const float ei = __shfl(e, min(i, 63));
+            if (i >= sp.n) continue;
             const f4 v = reinterpret_cast<const f4*>(sp.part_o + (r * sp.n + i) * D)[d];
 #pragma unroll
             for (int k = 0; k < 4; ++k) sum[k] = fmaf(v[k], ei, sum[k]);
