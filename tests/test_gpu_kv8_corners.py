@@ -8,6 +8,9 @@ from test_gpu_kv8 import Pair, rows
 
 pytestmark = pytest.mark.gpu
 
+# heads, K/V heads, head dim, rows: the kernel for many rows in each of its shapes (more than 512 groups of 16 columns x K/V heads)
+MANY = [(64, 64, 64, 129), (64, 64, 128, 300), (64, 64, 64, 600), (64, 64, 64, 700), (48, 48, 256, 200)]
+
 
 def towards(rng, x, q, lo, gap):
     """Keys [lo, end) of every K/V head get scores about `gap` above the others' for the head's first query."""
@@ -45,3 +48,19 @@ def test_newest_positions_of_a_long_cache(thk, ctx, H, Hkv, D, T, M):
     p.append(x, 0)
     p.check(q, T - M, decode=M == 1)
     p.check(q, T - M, mass=rng.random((Hkv, T + 3)).astype(np.float32), decode=M == 1)
+
+
+@pytest.mark.parametrize("H,Hkv,D,M", MANY + [(8, 8, 64, 3), (8, 2, 128, 1), (40, 1, 64, 4)])
+@pytest.mark.parametrize("fq,fk", [(2.0 ** -60, 2.0 ** -75), (2.0 ** -63, 2.0 ** -63), (2.0 ** -95, 2.0 ** -95), (2.0 ** -20, 2.0 ** -98)])
+def test_small_queries_and_keys(thk, ctx, H, Hkv, D, M, fq, fk):
+    """Queries and keys whose product leaves f32's range downwards: every score is 0, output and weights those of the mean."""
+    rng = np.random.default_rng(M + D)
+    n_past = 70
+    T = n_past + M
+    x, q = rows(rng, T, Hkv, D, spread=False), (rng.standard_normal((M, H, D)) * fq).astype(np.float32)
+    x[0] *= np.float32(fk)
+    p = Pair(thk, ctx, T + 1, H, Hkv, D)
+    p.append(x, 0)
+    mass = rng.random((Hkv, T + 1)).astype(np.float32)
+    p.check(q, n_past, mass=mass, decode=M == 1)
+    p.check(q, n_past, decode=M == 1)

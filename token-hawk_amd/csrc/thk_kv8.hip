@@ -1114,8 +1114,9 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
             const bool edge = t * kKv8Tile + kKv8Tile - 1 > a.n_past + wrow0;
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
-                // a block nobody sees has only -inf: its own factor may be NaN; and zero times -inf would be
-                const float kf = pos <= lim[k] && qf[k] * ks != 0.f ? qf[k] * ks : 1.f;
+                // A block nobody sees has only -inf: its own factor may be NaN; and zero times -inf would be.  Products below 2^-126 count as
+                // that: the sums they scale are below 2^30, so a score moves by 2^-96 at most.
+                const float kq = qf[k] * ks, kf = pos > lim[k] ? 1.f : kq < 0x1p-126f ? 0x1p-126f : kq;
                 if (edge) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[k][i >> 2][i & 3] = pos + i <= lim[k] ? s[k][i >> 2][i & 3] : -INFINITY;
@@ -1255,7 +1256,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_mass_tile_kernel
         load(min(c0 + 16 * W, cols - 1));                                      // without a branch: the next ones, or any
         const int row = min(c0 + n, cols - 1) / G, lim = c0 + n < cols ? a.n_past + row : -1;
         const bool edge = __any(tile * kKv8Tile + kKv8Tile - 1 > lim);
-        const float kf = pos <= lim && qf * ks != 0.f ? qf * ks : 1.f;     // a block this column does not see: no factor that could be NaN
+        const float kf = qf * ks;                                          // NaN at most in a block this column does not see: left out below
         float p[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
