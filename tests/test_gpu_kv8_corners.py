@@ -3,7 +3,7 @@ tests/kv8_ref.py; caches and their plain twins: test_gpu_kv8.py."""
 import numpy as np
 import pytest
 
-from kv8_ref import attention
+from kv8_ref import EPS, attention
 from test_gpu_kv8 import Pair, rows
 
 pytestmark = pytest.mark.gpu
@@ -64,3 +64,55 @@ def test_small_queries_and_keys(thk, ctx, H, Hkv, D, M, fq, fk):
     mass = rng.random((Hkv, T + 1)).astype(np.float32)
     p.check(q, n_past, mass=mass, decode=M == 1)
     p.check(q, n_past, decode=M == 1)
+
+
+def tops(rng, H, Hkv, D, M, n_past, gap, at):
+    """q and rows in which positions [at, at + 16) score about `gap` above all others, for every row and head."""
+    u = rng.standard_normal((Hkv, D))
+    G = H // Hkv
+    q = (np.repeat(u, G, 0)[None] + 0.1 * rng.standard_normal((M, H, D))).astype(np.float32)
+    x = rows(rng, n_past + M, Hkv, D, spread=False)
+    x[0] *= 0.1
+    x[0, at:at + 16] = u * (gap * np.sqrt(D) / (u * u).sum(1))[:, None]
+    return q, x
+
+
+@pytest.mark.parametrize("H,Hkv,D,M", MANY + [(8, 8, 64, 3), (8, 2, 128, 1)])
+@pytest.mark.parametrize("gap", [60, 82, 95, 250])
+def test_zero_values_under_the_top_scores(thk, ctx, H, Hkv, D, M, gap):
+    """The block with nearly all of the weight has zero values: the output is the others' small share, or nothing, and not NaN."""
+    rng = np.random.default_rng(M + gap)
+    n_past = 150
+    q, x = tops(rng, H, Hkv, D, M, n_past, gap, 16)
+    x[1, 16:32] = 0
+    p = Pair(thk, ctx, n_past + M, H, Hkv, D)
+    p.append(x, 0)
+    out, _ = p.attend(q, n_past)
+    eo, _, to, _ = attention(p.ref.values(), q, n_past)
+    assert np.all(np.abs(out - eo) <= to)
+    if gap == 60:                                                    # the small share is right, too, to its scores' error
+        share = np.linalg.norm(out.astype(np.float64) - eo) / np.linalg.norm(eo)
+        e = (D + 16) * EPS * np.abs(q).max() * np.abs(p.ref.values()[0]).sum(2).max() / np.sqrt(D)
+        assert share <= 2 * e + 1e-5, (share, e)
+
+
+@pytest.mark.parametrize("H,Hkv,D,M,n_past,lo", [(*m, 300, 128) for m in MANY])
+@pytest.mark.parametrize("big,gap", [(1e34, 200), (1e36, 200), (1e36, 81)])
+def test_large_values_of_next_to_no_weight(thk, ctx, H, Hkv, D, M, n_past, lo, big, gap):
+    """Values near the end of f32's range at positions of next to no weight: the product of the two is what counts, zero or not."""
+    rng = np.random.default_rng(M)
+    q, x = tops(rng, H, Hkv, D, M, n_past, gap, 16)
+    x[1, lo:lo + 64] *= np.float32(big)
+    p = Pair(thk, ctx, n_past + M, H, Hkv, D)
+    p.append(x, 0)
+    out, _ = p.attend(q, n_past)
+    val = p.ref.values()
+    eo, _, _, _ = attention(val, q, n_past)
+    apart = val.copy()                                               # the bound of either part by itself
+    apart[1, lo:lo + 64] = 0
+    _, _, to, _ = attention(apart, q, n_past)
+    e = (D + 16) * EPS * np.abs(q).max(2)[..., None] * np.repeat(np.abs(val[0]).sum(2).max(0), H // Hkv)[None, :, None] / np.sqrt(D)
+    share = attention(np.stack([val[0], np.abs(val[1]) - np.abs(apart[1])]), q, n_past)[0]
+    # the large values' part: weights good to their scores' error (twice) and to 2^-22 of the largest of their tile, whose 64 lie within a factor of 2
+    to = to + share * (2 * e + 400 * EPS)
+    assert np.all(np.abs(out - eo) <= to), float((np.abs(out - eo) / to).max())

@@ -947,7 +947,8 @@ __global__ __launch_bounds__(256) void kv8_attn_finish_kernel(Kv8Attn a, Kv8Spli
 //   q       scaled by a power of two per column so that its largest entry is in [2^14, 2^15): both parts stay far from f16's ends
 //   weights p * v_scale in units of 2^(ref - 15), ref >= the exponent of the largest weight the column has met (relative to its running
 //           maximum): at most 2^15, and what the lo part cannot hold is below 2^-40 of that largest weight.  The accumulators are rescaled
-//           only where the running maximum or ref moves, which a wave skips when none of its columns did.
+//           only where the running maximum or ref moves, which a wave skips when none of its columns did.  For ref p counts
+//           as 2^-113 at least, so that v_scale * 2^(15 - ref) is finite: what the lo part then loses, 2^-151 of the scale, f32's own p does not hold.
 // Bound by the matrix instructions and, beside them, the softmax's vector ones (on f16 the two do not overlap): 2048 rows over 6144 positions, 32
 // heads on 8, 420 us, 481 GFLOP of f16 products (the f32 work twice) at 1.15 PFLOP/s; a large f16 matrix product reaches 1.16.
 // S = 2: a second group of four waves takes every other tile, and its sums join the first's through LDS: 512 rows on 32 heads 18.8 -> 16.2 us.
@@ -1009,6 +1010,7 @@ __device__ __forceinline__ int xcd_order(int id, int n) {
     return x * q + (x < r ? x : r) + id / 8;
 }
 
+static const int kRefLeast = -126;                          // p * v_scale below f32's normal numbers: zero or no more than 2^15 units
 template <int D, int NC, int S>
 __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, int blocks, float scale) {
     constexpr int ST = D / 32, NG = D / 16, KF = 4 * ST, VF = 2 * NG, PIECES = (D / 64 * 4 + NG) / 4;      // f16 fragments of a tile; 16-byte pieces a thread stages
@@ -1058,7 +1060,7 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
         const bool valid = col < cols;
         lim[k] = valid ? a.n_past + col / G : T - 1;
         qf[k] = load_q_f16<D>(a.q + (valid ? (size_t)(col / G) * c.H + hkv * G + col % G : 0) * D + ch * 16, valid, qh[k], ql[k]) * scale;
-        m[k] = -INFINITY; l[k] = 0.f; ref[k] = -1000;
+        m[k] = -INFINITY; l[k] = 0.f; ref[k] = kRefLeast;
 #pragma unroll
         for (int g = 0; g < NG; ++g) o[k][g] = f4{0.f, 0.f, 0.f, 0.f};
     }
@@ -1133,11 +1135,11 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
                     ls += p[i];
                 }
                 const float vsu = pos <= lim[k] ? vs : 0.f;
-                const unsigned wm = chunks_max_bits(as_u(__builtin_amdgcn_exp2f(top - mu) * vsu));
+                const unsigned wm = chunks_max_bits(as_u(fmaxf(__builtin_amdgcn_exp2f(top - mu), 0x1p-113f) * vsu));
                 const int e = wm >= 0x7F800000u ? 1000 : wm == 0 ? -1000 : __builtin_amdgcn_frexp_expf(as_f(wm));
                 if (__any(mn != m[k] || e > ref[k])) {                      // NaN maxima compare unequal: rescaled each time, harmless
                     const float al = __builtin_amdgcn_exp2f(m[k] - mu);
-                    const int shrunk = ref[k] + (al > 0.f ? __builtin_amdgcn_frexp_expf(al) - 1 : -1000), rn = max(max(shrunk, e), -1000);
+                    const int shrunk = ref[k] + (al > 0.f ? __builtin_amdgcn_frexp_expf(al) - 1 : -1000), rn = max(max(shrunk, e), kRefLeast);
                     const float f = ldexpf(al, max(min(ref[k] - rn, 2000), -2000));
 #pragma unroll
                     for (int g = 0; g < NG; ++g)
