@@ -96,7 +96,8 @@ def test_zero_values_under_the_top_scores(thk, ctx, H, Hkv, D, M, gap):
         assert share <= 2 * e + 1e-5, (share, e)
 
 
-@pytest.mark.parametrize("H,Hkv,D,M,n_past,lo", [(*m, 300, 128) for m in MANY])
+# the kernel for few rows: the same wave's next tile; the one for many rows: any
+@pytest.mark.parametrize("H,Hkv,D,M,n_past,lo", [(*m, 300, 128) for m in MANY] + [(32, 32, 64, 70, 1200, 512), (64, 32, 128, 33, 1200, 512), (32, 32, 256, 65, 900, 256)])
 @pytest.mark.parametrize("big,gap", [(1e34, 200), (1e36, 200), (1e36, 81)])
 def test_large_values_of_next_to_no_weight(thk, ctx, H, Hkv, D, M, n_past, lo, big, gap):
     """Values near the end of f32's range at positions of next to no weight: the product of the two is what counts, zero or not."""

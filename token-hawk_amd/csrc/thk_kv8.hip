@@ -736,9 +736,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_attn_split_kerne
         for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(s[i] - mu); ls += s[i]; }
         l += ls;
         // weights p * vs in steps of 2^(e - 22), e the exponent of the tile's largest: whole numbers below 2^22.  Blocks no row of this
-        // column sees (p = 0 throughout) must not bring in their scale, which may be NaN.
+        // column sees (p = 0 throughout) must not bring in their scale, which may be NaN.  For e p counts as 2^-106 at least: vs in these steps stays finite.
         const float vsu = pos <= lim ? vs : 0.f;
-        const float wm = as_f(chunks_max_bits(as_u(__builtin_amdgcn_exp2f(sm - mu) * vsu)));
+        const float wm = as_f(chunks_max_bits(as_u(fmaxf(__builtin_amdgcn_exp2f(sm - mu), 0x1p-106f) * vsu)));
         const int e = __builtin_amdgcn_frexp_expf(wm);
         const float fac = ldexpf(vsu, 22 - e), f = ldexpf(1.f, e - 22) + (wm - wm);                  // wm - wm: 0, or NaN if wm is not finite
         i4 pd[3];
