@@ -117,3 +117,24 @@ def test_large_values_of_next_to_no_weight(thk, ctx, H, Hkv, D, M, n_past, lo, b
     # the large values' part: weights good to their scores' error (twice) and to 2^-22 of the largest of their tile, whose 64 lie within a factor of 2
     to = to + share * (2 * e + 400 * EPS)
     assert np.all(np.abs(out - eo) <= to), float((np.abs(out - eo) / to).max())
+
+
+@pytest.mark.parametrize("H,Hkv,D,M", MANY + [(8, 8, 64, 3), (8, 2, 128, 1), (4, 1, 64, 9)])
+@pytest.mark.parametrize("down", [60, 100])
+def test_values_near_the_least_block(thk, ctx, H, Hkv, D, M, down):
+    """Values down to 2^-100, the least a block holds, under flat scores: as good, relative to them, as ordinary ones (a power of two changes no code)."""
+    rng = np.random.default_rng(M + D)
+    n_past = 2007
+    x, q = rows(rng, n_past + M, Hkv, D, spread=False), (0.01 * rng.standard_normal((M, H, D))).astype(np.float32)
+    p = Pair(thk, ctx, n_past + M, H, Hkv, D)
+    p.append(x, 0)
+    val = p.ref.values()
+    one, _ = p.attend(q, n_past)
+    x[1] *= np.float32(2.0 ** -down)
+    p.append(x, 0)
+    assert np.array_equal(p.ref.values()[1], val[1] * np.float32(2.0 ** -down))
+    out, _ = p.attend(q, n_past)
+    # a power of two changes no rounding above 2^-126; below, sums are rounded to 2^-149: once a tile of 64 and part, and at the end
+    least = (n_past + M) / 16 * 2.0 ** -150 * 2.0 ** down
+    off = np.abs(out.astype(np.float64) * 2.0 ** down - one)
+    assert np.all(off <= 4 * EPS * np.abs(one) + least), float((off / (4 * EPS * np.abs(one) + least)).max())

@@ -1211,9 +1211,14 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
         const int col = wcol0 + 16 * k + n;
         if (col >= cols) continue;
         const size_t r = (size_t)(col / G) * c.H + hkv * G + col % G;
-        const float lt = chunks_sum(l[k]), f = ldexpf(1.f, max(ref[k], -200) - 15) / lt;
+        const float lt = chunks_sum(l[k]), inv = 1.f / lt;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) *reinterpret_cast<f4*>(a.out + r * D + 16 * g + 4 * ch) = o[k][g] * f;
+        for (int g = 0; g < NG; ++g) {                                     // the unit last: with 1 / sum it may leave the normal numbers where the output does not
+            f4 v = o[k][g] * inv;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = ldexpf(v[i], ref[k] - 15);
+            *reinterpret_cast<f4*>(a.out + r * D + 16 * g + 4 * ch) = v;
+        }
         if (a.ml && ch == 0) a.ml[r] = float2{m[k], lt};
     }
 }
