@@ -138,3 +138,46 @@ def test_values_near_the_least_block(thk, ctx, H, Hkv, D, M, down):
     least = (n_past + M) / 16 * 2.0 ** -150 * 2.0 ** down
     off = np.abs(out.astype(np.float64) * 2.0 ** down - one)
     assert np.all(off <= 4 * EPS * np.abs(one) + least), float((off / (4 * EPS * np.abs(one) + least)).max())
+
+
+@pytest.mark.parametrize("H,Hkv,D,M", MANY)
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_many_rows_nan_reaches_only_rows_that_see_it(thk, ctx, H, Hkv, D, M, what):
+    rng = np.random.default_rng(M + D)
+    n_past, at, head = 20, 20 + M // 2, 5
+    T = n_past + M
+    x = rows(rng, T + 40, Hkv, D)
+    x[1 if what == "v" else 0, at, head, 3] = np.nan
+    x[:, T:] = np.nan                                                # and in the blocks behind the last position's
+    p = Pair(thk, ctx, T + 40, H, Hkv, D)
+    p.append(x[:, :T], 0)
+    if T % 16 == 0:
+        p.append(x[:, T:], T)
+    else:
+        p.append(x[:, T + 16 - T % 16:], T + 16 - T % 16)
+    q, mass = rng.standard_normal((M, H, D)).astype(np.float32), rng.random((Hkv, T + 40)).astype(np.float32)
+    out, m = p.attend(q, n_past, mass)
+    first = at // 16 * 16                                            # the block's first position: the first row that sees it
+    bad = (np.arange(M)[:, None] + n_past >= first) & (np.arange(H) == head)[None]
+    assert np.array_equal(np.isnan(out).all(2), bad) and np.array_equal(np.isnan(out).any(2), bad)
+    val = p.ref.values(0, T)
+    val[1 if what == "v" else 0, first:first + 16, head] = 0
+    eo, em, to, tm = attention(val, q, n_past, mass)
+    assert np.all((np.abs(out - eo) <= to)[~bad])
+    if what == "v":                                                  # the weights do not know of it
+        assert np.all(np.abs(m[:, :T] - em) <= tm)
+    else:
+        nan = np.zeros((Hkv, T), bool)
+        nan[head] = True
+        assert np.array_equal(np.isnan(m[:, :T]), nan) and np.all((np.abs(m[:, :T] - em) <= tm)[~nan])
+    assert np.all(m[:, T:] == 7.0)
+
+
+def test_many_rows_in_slabs(thk, ctx):
+    """Two launches of the kernel for many rows and a last one of few: weights of later slabs add to earlier ones'."""
+    rng = np.random.default_rng(31)
+    H, D, n_past = 8, 64, 33
+    for M in (2048 + 1100, 4096 + 21):
+        p = Pair(thk, ctx, n_past + M + 3, H, H, D)
+        p.append(rows(rng, n_past + M, H, D), 0)
+        p.check(rng.standard_normal((M, H, D)).astype(np.float32), n_past, mass=rng.random((H, n_past + M + 3)).astype(np.float32))
