@@ -355,9 +355,11 @@ int thk_peer_memory_kind(const thk_peer* p);             /* THK_PEER_MEM_* of th
 int thk_peer_destroy(thk_peer* p);
 
 /* ---------------------------------------------------------------- 8-bit K/V cache
- * One layer's K/V cache of one sequence, held as 8-bit codes with a scale for every block of THK_KV8_BLOCK positions and K/V head: a quarter
- * of the f32 cache's bytes (thk_kv_append / thk_attn_decode / thk_attn_prefill), attention that reads the codes, and eviction by the
- * attention weight a position has drawn.  The reference keeps an f32 cache and ends when it is full (th-llama-loader.cpp:335).
+ * One layer's K/V cache of one sequence, held as 8-bit codes with a scale for every block of THK_KV8_BLOCK positions and K/V head,
+ * attention that reads the codes, and eviction by the attention weight a position has drawn.  Beside thk_kv_append, thk_attn_decode and
+ * thk_attn_prefill: codes and scales take a quarter of their f32 cache's bytes; with the open block's rows and the workspace of the calls it is
+ * 26 % (16384 positions, 32 heads of 128), 29 % (512) or 33 % (512, 32 heads on 8), more for shorter caches: thk_kv8_bytes says how many.
+ * The reference keeps an f32 cache and ends when it is full (th-llama-loader.cpp:335).
  *   block   positions [16 b, 16 b + 16) of one K/V head; amax = the largest magnitude in its rows (the positions appended so far)
  *   scale   f32(amax / 127);  code = rint(x * f32(127 / amax)), the exact product rounded once, ties to even;  value = f32(code * scale)
  *           amax < 2^-100: the block is zero.  A NaN or an infinity in a block makes its scale NaN: rows that may see one of its positions

@@ -37,7 +37,11 @@ hipError_t launch_kv8_select(int Hkv, int T, int keep, int sink, int recent, con
 }
 hipError_t launch_kv8_move(const Kv8View&, const Kv8View&, int keep, const int32_t*, hipStream_t) { note("move %d", keep); return launched(); }
 hipError_t launch_kv8_attn_tile(const Kv8Attn& a, hipStream_t) { note("tile %d %d", a.n_past, a.M); return launched(); }
-hipError_t launch_kv8_attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t) { note("split %d %d %d", a.n_past, a.M, sp.n); return launched(); }
+hipError_t launch_kv8_attn_split(const Kv8Attn& a, const Kv8Split& sp, hipStream_t) {
+    const size_t rows = (size_t)a.M * a.c.H * (sp.n > 1 ? sp.n : 0);       // parts and statistics have to fit between their arrays' starts
+    if ((const char*)(sp.part_o + rows * a.c.D) > (const char*)sp.part_ml || (a.ml && (const char*)(a.ml + (size_t)a.M * a.c.H) > (const char*)sp.part_o)) return hipErrorOutOfMemory;
+    if (sp.counters ? (const char*)(sp.part_ml + rows) > (const char*)sp.counters : sp.scores && (const char*)(sp.part_ml + rows) > (const char*)sp.scores) return hipErrorOutOfMemory;
+    note("split %d %d %d", a.n_past, a.M, sp.n); return launched(); }
 hipError_t launch_kv8_attn_mass(const Kv8Attn& a, hipStream_t) { note("mass %d %d %d%s", a.n_past, a.M, a.mass_n, a.mass_in == a.mass_out ? " in place" : ""); return launched(); }
 }
 

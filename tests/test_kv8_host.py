@@ -142,3 +142,42 @@ def test_launches_run_on_the_contexts_device_and_errors_come_back(lib):
         assert call() == HIP and lib.stub_device() == 1
     lib.stub_set(1, 0, 0, 0)
     assert lib.thk_kv8_destroy(kv) == 0 and lib.thk_kv8_destroy(to) == 0 and lib.stub_device() == 1
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 1, 64), (64, 8, 8, 64), (512, 32, 32, 128), (512, 32, 8, 128), (2048, 40, 40, 128), (4096, 32, 8, 128), (16384, 32, 32, 128), (131072, 64, 8, 256)])
+def test_size_is_that_of_its_calls(env, lib, shape):
+    """Codes, scales, the open blocks' rows, and a workspace for no more rows and parts than calls on a cache of this length can have."""
+    n_ctx, H, Hkv, D = shape
+    h = env.create(*shape)
+    n = -(-n_ctx // 128) * 128
+    cache = 2 * Hkv * n * D + 2 * Hkv * n // 16 * 4 + 2 * Hkv * 16 * D * 4
+    cut = -(-n_ctx // 64) > (4 if D == 256 else 8)                     # more than a tile of 64 for every wave of a workgroup: parts
+    rows = 8192 if n_ctx > 32768 else 4096 if cut else 0
+    work = min(n_ctx, 2048) * H * 8 + rows * (D * 4 + 8) + 512 * 4 + (H * n * 4 if H // Hkv <= 16 else 0)
+    assert cache + work <= lib.thk_kv8_bytes(h) <= cache + work + 6 * 256
+    assert lib.thk_kv8_destroy(h) == 0
+
+
+@pytest.mark.parametrize("shape,percent", [((512, 32, 32, 128), 30), ((512, 32, 8, 128), 34), ((2048, 40, 40, 128), 30), ((16384, 32, 32, 128), 27)])
+def test_size_against_the_f32_cache(env, lib, shape, percent):
+    """By the sum above: 29.4, 32.9, 29.5 and 26.0 % of the f32 cache."""
+    n_ctx, _, Hkv, D = shape
+    h = env.create(*shape)
+    assert lib.thk_kv8_bytes(h) * 100 < percent * 2 * 4 * n_ctx * Hkv * D
+    assert lib.thk_kv8_destroy(h) == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_calls_fit_the_workspace(env, lib, D):
+    """Every size of cache and call: the parts and row statistics of a launch lie inside the cache's memory (the stand-in launch checks it)."""
+    far = 1 << 40
+    for n_ctx in (1, 16, 63, 64, 65, 257, 513, 1025, 5000, 33000, 131072):
+        for H, Hkv in ((1, 1), (8, 8), (32, 8), (17, 1), (40, 40), (64, 2), (256, 128), (257, 257), (600, 600), (1024, 1)):
+            kv = env.create(n_ctx, H, Hkv, D)
+            for M in (1, 2, 3, 16, 17, 31, 64, 100, 257, 1000, 2048, 2049):
+                for T in {M, (M + n_ctx) // 2, n_ctx}:
+                    if M <= T <= n_ctx:
+                        for mass in (None, far):
+                            assert lib.thk_kv8_attn_prefill(kv, 2 * far, T - M, M, mass, mass, 3 * far) == 0, (n_ctx, H, Hkv, M, T)
+            assert lib.thk_kv8_destroy(kv) == 0
+            lib.stub_log()

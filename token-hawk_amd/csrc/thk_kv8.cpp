@@ -12,6 +12,7 @@ struct thk_kv8 {
     float2* ml = nullptr;       // per-row softmax statistics of an attention call that counts weights
     float* part_o = nullptr;    // parts of rows that are split over the positions
     float2* part_ml = nullptr;
+    int64_t part_rows = 0;      // rows x parts they hold; the selection of long sets uses part_o too
     unsigned* counters = nullptr;
     float* scores = nullptr;    // [H][padded n_ctx]: a single row's scores, for the weight count (groups of up to kKv8ScoredHeads heads)
 };
@@ -30,6 +31,11 @@ struct DeviceScope {
 bool overlap(const void* a, size_t na, const void* b, size_t nb) { return a && b && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+// Parts that T positions are cut into at most: a tile for every wave, no more than one wave joins.
+int64_t max_parts(int64_t T, int64_t D) {
+    const int64_t tiles = (T + kKv8Tile - 1) / kKv8Tile, waves = kv8_split_waves((int)D);
+    return std::min<int64_t>((tiles + waves - 1) / waves, 64);
+}
 
 // An allocation, a free or a blocking call inside a stream capture would break the capture: refused before anything is touched.
 int refuse_capture(thk_ctx* ctx, const char* what) {
@@ -57,9 +63,12 @@ extern "C" int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_
     v.n_blk = (int)((n_ctx + kKv8Pad - 1) / kKv8Pad) * (kKv8Pad / kKv8Block);
     v.H = (int)H; v.Hkv = (int)H_kv; v.D = (int)D;
     const size_t codes = (size_t)H_kv * v.n_blk * kKv8Block * D, scales = up256((size_t)H_kv * v.n_blk * 4), tail = (size_t)2 * H_kv * kKv8Block * D * 4;
-    const size_t at = up256((size_t)2 * H_kv * sizeof(int2)), ml = (size_t)kKv8RowSlab * H * sizeof(float2);
-    const size_t part = (size_t)kKv8SplitRows * (D * 4 + sizeof(float2)), scores_bytes = H / H_kv <= kKv8ScoredHeads ? (size_t)H * v.n_blk * kKv8Block * 4 : 0;
-    kv->mem_bytes = 2 * codes + 2 * scales + tail + at + ml + part + kKv8Groups * 4 + scores_bytes;
+    // The workspace is what calls on this cache can ask for: no more rows than positions, no more parts than its length is cut into.
+    const int64_t rows = n_ctx < kKv8RowSlab ? n_ctx : kKv8RowSlab, parts = max_parts(n_ctx, D);
+    kv->part_rows = n_ctx > kKv8SliceFrom ? kKv8SliceRows : parts > 1 ? std::min<int64_t>(kKv8SplitRows, parts * rows * H) : 0;
+    const size_t at = up256((size_t)2 * H_kv * sizeof(int2)), ml = up256((size_t)rows * H * sizeof(float2)), part_o = (size_t)kv->part_rows * D * 4;
+    const size_t part_ml = up256((size_t)kv->part_rows * sizeof(float2)), scores_bytes = H / H_kv <= kKv8ScoredHeads ? (size_t)H * v.n_blk * kKv8Block * 4 : 0;
+    kv->mem_bytes = 2 * codes + 2 * scales + tail + at + ml + part_o + part_ml + kKv8Groups * 4 + scores_bytes;
     hipError_t e = hipMalloc(&kv->mem, kv->mem_bytes);
     if (e != hipSuccess) {
         (void)hipGetLastError();
@@ -75,8 +84,8 @@ extern "C" int thk_kv8_create(thk_ctx* ctx, int64_t n_ctx, int64_t H, int64_t H_
     v.tail = (float*)p; p += tail;
     v.tail_at = (int2*)p; p += at;
     kv->ml = (float2*)p; p += ml;
-    kv->part_o = (float*)p; p += (size_t)kKv8SplitRows * D * 4;
-    kv->part_ml = (float2*)p; p += (size_t)kKv8SplitRows * sizeof(float2);
+    kv->part_o = (float*)p; p += part_o;
+    kv->part_ml = (float2*)p; p += part_ml;
     kv->counters = (unsigned*)p; p += kKv8Groups * 4;
     kv->scores = (float*)p;
     e = hipMemsetAsync(kv->mem, 0, kv->mem_bytes, ctx->stream);
@@ -153,9 +162,8 @@ static int kv8_attention(thk_kv8* kv, const char* what, const float* q, int64_t 
         // rows: no past, 512 groups 11.2 and 10.7 us, 768 17.6 and 12.9; over 1024 positions 22.6 and 29.3, 34.2 and 32.3; over 8192 91 and 148, 138 and 155.
         if (groups <= kKv8Groups) {
             Kv8Split sp{};
-            const int64_t T = a.n_past + a.M, tiles = (T + kKv8Tile - 1) / kKv8Tile, waves = kv8_split_waves(a.c.D);
-            // one workgroup on every CU, at least a tile for every wave
-            const int64_t n = std::min({256 / groups, (tiles + waves - 1) / waves, (int64_t)64, kKv8SplitRows / ((int64_t)a.M * a.c.H)});
+            const int64_t T = a.n_past + a.M;
+            const int64_t n = std::min(256 / groups, max_parts(T, a.c.D));              // one workgroup on every CU
             sp.n = n < 1 ? 1 : (int)n; sp.part_o = kv->part_o; sp.part_ml = kv->part_ml;
             sp.stream = cg == 1 && 2 * T * a.c.Hkv * a.c.D >= (64 << 20);  // twice what the L2s hold: 112 -> 100 us at 65535 x 32 heads; at 2047 x 40 heads 10.4 -> 11.1
             // Joined inside the launch where the last workgroup has little to do: 4096 positions, 32 heads on 8, 10.4 -> 9.7 us, at 8192 10.8 -> 11.3; and
@@ -201,7 +209,7 @@ extern "C" int thk_kv8_evict(thk_kv8* src, int64_t T, int64_t n_keep, int64_t n_
     DeviceScope dev(ctx->device);
     HIPCHK(ctx, dev.err);
     HIPCHK(ctx, launch_kv8_select(src->view.Hkv, (int)T, (int)n_keep, (int)n_sink, (int)n_recent, mass_in, src->n_ctx, mass_out, dst->n_ctx, kept,
-                                  reinterpret_cast<unsigned*>(src->part_o), (int64_t)kKv8SplitRows * src->view.D, ctx->stream));
+                                  reinterpret_cast<unsigned*>(src->part_o), src->part_rows * src->view.D, ctx->stream));
     HIPCHK(ctx, launch_kv8_move(src->view, dst->view, (int)n_keep, kept, ctx->stream));
     return THK_OK;
 }

@@ -1333,7 +1333,7 @@ hipError_t launch_kv8_read(const Kv8View& c, int64_t pos, int64_t n, float* k_ou
 hipError_t launch_kv8_select(int Hkv, int T, int n_keep, int n_sink, int n_recent, const float* mass_in, int64_t ld_in, float* mass_out, int64_t ld_out, int32_t* kept,
                              unsigned* work, int64_t work_words, hipStream_t st) {
     const int64_t slices = std::min((T + 4095) / 4096, (int)std::min<int64_t>(work_words / (Hkv * kKv8SliceWords), 64));
-    if (T > 32768 && slices >= 2) {
+    if (T > kKv8SliceFrom && slices >= 2) {
         const int n = (int)slices, slice = ((T + n - 1) / n + 3) & ~3;
         Slices s{work, work + (size_t)3 * Hkv * n * 2048, nullptr};
         s.picks = s.above + (size_t)2 * Hkv * n;

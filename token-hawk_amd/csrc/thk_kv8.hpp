@@ -8,7 +8,9 @@ namespace thk {
 static const int kKv8Block = 16;      // positions that share one K scale and one V scale per K/V head
 static const int kKv8Tile = 64;       // positions one step of the split attention kernel takes
 static const int kKv8Pad = 128;       // a cache holds whole multiples of this many positions: no kernel's step reads behind it
-static const int kKv8SplitRows = 8192; // rows x splits whose parts the workspace holds
+static const int kKv8SplitRows = 4096; // rows x parts a launch has at most: 16 columns of 256 workgroups
+static const int kKv8SliceFrom = 32768; // positions above which the selection may go in slices
+static const int kKv8SliceRows = 8192; // rows of D words a cache that long keeps for the slices' counts: 5 slices at 32 heads of 128, 10 at 16
 static const int kKv8Groups = 512;    // column groups x K/V heads up to which the positions are split (and counters there are)
 static const int kKv8SliceWords = 3 * 2048 + 16; // what the selection of long sets keeps for a slice of a head, in words
 static const int kKv8ScoredHeads = 16; // query heads of a K/V head up to which a single row's scores are kept for the weight count (else they are computed again)
