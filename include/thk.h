@@ -365,6 +365,9 @@ int thk_peer_destroy(thk_peer* p);
  *           amax < 2^-100: the block is zero.  A NaN or an infinity in a block makes its scale NaN: rows that may see one of its positions
  *           get NaN, others do not (K: through the score; V: in the output only, the weights stay).
  *   grouped heads: query head h reads K/V head h / (H / H_kv).
+ *   bits    sums, statistics and scales are f32.  In the products a head's row of q is held to 22 bits of its largest entry (a row below 2^-100 counts
+ *           as zero), a softmax weight times its V scale to 21 or 22 bits of the largest in a tile of 64 positions or of the row.
+ *   ranges  max|q| max|k| D and T max|v| have to stay below 2^127, as f32 sums of them have to: beyond, outputs may be infinite or NaN.
  * The cache does not count positions: the caller passes them, as for thk_kv_append, and has appended [0, T) before it attends to T.  Calls are
  * stream-ordered, allocate nothing and may be captured into a graph (create and destroy may not); a replay uses the captured positions and
  * pointers.  The cache owns the workspace of its calls: calls and replays of ONE cache must not overlap on two streams.

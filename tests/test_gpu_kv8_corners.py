@@ -174,10 +174,10 @@ def test_many_rows_nan_reaches_only_rows_that_see_it(thk, ctx, H, Hkv, D, M, wha
 
 
 def test_many_rows_in_slabs(thk, ctx):
-    """Two launches of the kernel for many rows and a last one of few: weights of later slabs add to earlier ones'."""
+    """Launches of the kernel for many rows and a last one of few, or of one: weights of later slabs add to earlier ones'."""
     rng = np.random.default_rng(31)
     H, D, n_past = 8, 64, 33
-    for M in (2048 + 1100, 4096 + 21):
+    for M in (2048 + 1, 2048 + 1100, 4096 + 21):
         p = Pair(thk, ctx, n_past + M + 3, H, H, D)
         p.append(rows(rng, n_past + M, H, D), 0)
         p.check(rng.standard_normal((M, H, D)).astype(np.float32), n_past, mass=rng.random((H, n_past + M + 3)).astype(np.float32))

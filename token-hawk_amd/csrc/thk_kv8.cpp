@@ -160,6 +160,7 @@ static int kv8_attention(thk_kv8* kv, const char* what, const float* q, int64_t 
         const int64_t G = a.c.H / a.c.Hkv, cols = a.M * G, cg = (cols + 15) / 16, groups = cg * a.c.Hkv;      // workgroups without a split
         // Few columns: split over the positions, a tile of 64 a wave in turn; many: whole rows, tiles shared by a workgroup.  32 heads of 128, split and
         // rows: no past, 512 groups 11.2 and 10.7 us, 768 17.6 and 12.9; over 1024 positions 22.6 and 29.3, 34.2 and 32.3; over 8192 91 and 148, 138 and 155.
+        // The rule does not look at the length: 768 groups over 8192 positions would be 17 us faster split.
         if (groups <= kKv8Groups) {
             Kv8Split sp{};
             const int64_t T = a.n_past + a.M;

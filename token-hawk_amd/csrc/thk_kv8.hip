@@ -512,14 +512,16 @@ static const float kLog2e = 1.44269504088896340736f;      // scores carry log2(e
 // v_mfma_i32_16x16x64_i8 with the cache's codes as they are - no conversion - and the f32 operand (q, then the weights) as a fixed-point
 // number of three balanced base-256 digits: x = d2 2^16 + d1 2^8 + d0, each digit an i8 operand of its own product, the three i32 sums
 // exact.  q is fixed relative to its column's largest entry (23 bits with the sign), the weights p * v_scale relative to the largest of their column
-// in the tile of 64 positions (a power of two, 21 to 22 bits): errors stay at f32's own.
+// in the tile of 64 positions (a power of two, 21 to 22 bits).  Both lie above f32's own rounding, which short sums show (64 positions 6.7e-7 from the
+// 64-bit result in norm, elementary f32 operations 3.5e-7); over 2047 positions the two are alike, over 65535 the fewer f32 additions count (8.7e-7, 2.2e-6).
 // Operand layout (A: row = lane % 16, B: column = lane % 16, both 16 consecutive k per lane of chunk lane / 16; result: column lane % 16,
 // rows 4 (lane / 16) + i).  The k order is free as long as A and B share it, and the row order of the first product is chosen so that
 // lane chunk c ends up with the scores of the 16 positions of block c: then one K scale and one V scale per lane serve a whole tile, and
 // the second product's B operand is what the lane already holds - no exchange between lanes.
 // Long caches are bound by memory: 65535 positions on 32 heads, 537 MB in 89 us (6.0 TB/s; the bare reads in this pattern reach 6.9), 131071 on 8
-// heads for 64 query heads 47 us with the joining launch.  Short ones are a chain of latencies (launch, load, one or two tiles, join of the waves,
-// join of the splits): 64 positions 4.2 us, 512 on 32 heads with weights 8.0 us, 2047 on 40 heads 9.4 us.
+// heads for 64 query heads 47 us with the joining launch.  Short ones are a chain of latencies (launch, load, one tile, join of the waves, from 513
+// positions on join of the parts): 64 positions 4.4 us, 512 on 32 heads with weights 8.0 us (one part, 32 workgroups: 224 CUs have nothing to do),
+// 2047 on 40 heads 9.7 us.
 typedef int i4 __attribute__((ext_vector_type(4)));
 struct U2 { unsigned a, b; };
 // Between them, a and b hold a value and that of the lane 16 (32) away, in every lane.  The swap works on two registers: the empty asm keeps
@@ -1226,8 +1228,9 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
 // ---------------------------------------------------------------- weight count of many rows
 // mass_out = mass_in + sum over the columns of exp2(s - m) / l.  A workgroup takes 64 positions; its W waves share the columns, 16 at a time
 // in turn, each with the K fragments of all 64 positions in registers and the next columns' q on the way; the waves' sums are added in a
-// fixed order.  Scores anew instead of kept ones: [rows][heads][positions] would be hundreds of times the cache.  Bound by vector instructions (a
-// column's digits, 16 exponentials a lane): 512 rows on 32 heads 15 us, of which the first tile's workgroup, all rows' columns, is the longest.
+// fixed order.  Scores anew instead of kept ones: [rows][heads][positions] would be hundreds of times the cache.  512
+// rows on 32 heads 13 us (15 in a trace), one workgroup a CU: its first tile's, with all rows' columns, has 1.8 times the mean to do and is what the
+// launch takes.  The vector instructions are 4.0 us of it on even load; waves wait 44 % of their cycles.
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_mass_tile_kernel(Kv8Attn a, float scale) {
     constexpr int KC = D / 64;

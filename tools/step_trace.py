@@ -4,7 +4,7 @@
 Needs the -DTHK_TRACE build: python -c "import __graft_entry__ as g; g.build_libthk(trace=True)" -> token-hawk_amd/libthk_trace.so
     THK_LIB=token-hawk_amd/libthk_trace.so python tools/step_trace.py [7b|13b] [name=value ...]
 
-Every wave stamps s_memrealtime (100 MHz, scalar instructions only) at: kernel entry | activation vector staged in LDS | first weight
+Every wave stamps s_memrealtime (100 MHz; read by a scalar instruction, written by lane 0 with a vector store) at: kernel entry | activation vector staged in LDS | first weight
 batch consumed | done.  Per launch kind (averaged over layers 1..), all in microseconds:
   gap       first workgroup entry - last workgroup done of the PREVIOUS launch (the boundary)
   ramp      last workgroup entry - first workgroup entry (dispatch)
