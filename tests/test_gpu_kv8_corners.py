@@ -181,3 +181,35 @@ def test_many_rows_in_slabs(thk, ctx):
         p = Pair(thk, ctx, n_past + M + 3, H, H, D)
         p.append(rows(rng, n_past + M, H, D), 0)
         p.check(rng.standard_normal((M, H, D)).astype(np.float32), n_past, mass=rng.random((H, n_past + M + 3)).astype(np.float32))
+
+
+# the many-rows kernel, a single row and few rows, one and several tiles a wave and parts
+LARGE = MANY + [(8, 8, 64, 3), (8, 2, 128, 1), (40, 1, 64, 4), (300, 300, 64, 1)]
+
+
+def one_hot(rng, thk, ctx, H, Hkv, D, M, n_past, big):
+    """Scores around `big` and more, one position's above the next by more than that for every row -> cache, q, the position."""
+    T, at = n_past + M, 37
+    x = rows(rng, T, Hkv, D, spread=False)
+    u = rng.standard_normal((Hkv, D))
+    x[0] *= np.float32(big ** 0.5)
+    x[0, at] = u * 20 * big ** 0.5
+    q = (np.repeat(u, H // Hkv, 0)[None] * (1 + rng.random((M, 1, 1))) * big ** 0.5).astype(np.float32)
+    p = Pair(thk, ctx, T, H, Hkv, D)
+    p.append(x, 0)
+    k = p.ref.values()[0].astype(np.float64)
+    for j in range(Hkv):
+        s = np.sort(q[:, j * (H // Hkv)].astype(np.float64) @ k[:, j].T / np.sqrt(D), 1)
+        assert np.all(s[:, -1] - s[:, -2] > big)
+    return p, q, at
+
+
+@pytest.mark.parametrize("H,Hkv,D,M", LARGE)
+@pytest.mark.parametrize("big,n_past", [(1e7, 90), (1e9, 90), (1e12, 90), (1e9, 1400)])
+def test_scores_beyond_the_steps_of_f32(thk, ctx, H, Hkv, D, M, big, n_past):
+    """Scores so large that f32 tells them apart by no less than 1 to 10^5: a row's weight is on its single largest one, whatever that was rounded to."""
+    p, q, at = one_hot(np.random.default_rng(M + D), thk, ctx, H, Hkv, D, M, n_past, big)
+    out, _ = p.attend(q, n_past, None, decode=M == 1)
+    want = np.repeat(p.ref.values()[1, at], H // Hkv, 0)[None]
+    # one weight of 1: held to 22 bits, its value by one product and one quotient
+    assert np.all(np.abs(out - want) <= 16 * EPS * np.abs(want).max()), float(np.abs(out - want).max())

@@ -507,6 +507,13 @@ __global__ __launch_bounds__(256) void kv8_move_kernel(Kv8View s, Kv8View d, int
 
 static const float kLog2e = 1.44269504088896340736f;      // scores carry log2(e): the weights are exp2
 
+// a * b rounded to f32, whatever it goes to: a score has to be the same number where it is compared and where the maximum is taken from it.
+// Fused into the difference, the largest one's weight would be 2^(half a step of the maximum) and not 1.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
 // ---------------------------------------------------------------- attention of few rows: i8 matrix instructions, split over the positions
 // out_n = sum_t p_nt v_t with p = softmax(q_n . k_t), for up to 16 (row, head) columns n that read one K/V head.  Both products run on
 // v_mfma_i32_16x16x64_i8 with the cache's codes as they are - no conversion - and the f32 operand (q, then the weights) as a fixed-point
@@ -703,7 +710,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_attn_split_kerne
                 for (int kc = 0; kc < KC; ++kc) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[g][kc], qd[d][kc], acc[d], 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * g + i] = join_digits(acc[2][i], acc[1][i], acc[0][i]) * kf;
+            for (int i = 0; i < 4; ++i) s[4 * g + i] = rounded_product(join_digits(acc[2][i], acc[1][i], acc[0][i]), kf);
             if (g & 1) __builtin_amdgcn_sched_barrier(0);            // two groups in flight: more only cost registers
         }
         if (decltype(more)::value) load_k(t + W);
@@ -1128,12 +1135,12 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
                 float top = s[k][0][0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) top = fmaxf(top, s[k][i >> 2][i & 3]);
-                top *= kf;
+                top = rounded_product(top, kf);
                 const float mn = fmaxf(m[k], chunks_max(top)), mu = mn == -INFINITY ? 0.f : mn;
                 float p[16], ls = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    p[i] = __builtin_amdgcn_exp2f(fmaf(s[k][i >> 2][i & 3], kf, -mu));
+                    p[i] = __builtin_amdgcn_exp2f(rounded_product(s[k][i >> 2][i & 3], kf) - mu);
                     ls += p[i];
                 }
                 const float vsu = pos <= lim[k] ? vs : 0.f;
