@@ -213,3 +213,16 @@ def test_scores_beyond_the_steps_of_f32(thk, ctx, H, Hkv, D, M, big, n_past):
     want = np.repeat(p.ref.values()[1, at], H // Hkv, 0)[None]
     # one weight of 1: held to 22 bits, its value by one product and one quotient
     assert np.all(np.abs(out - want) <= 16 * EPS * np.abs(want).max()), float(np.abs(out - want).max())
+
+
+@pytest.mark.parametrize("H,Hkv,D,M", LARGE)
+@pytest.mark.parametrize("big,n_past", [(1e7, 90), (1e9, 90), (1e12, 90), (1e9, 1400)])
+def test_weights_of_scores_beyond_the_steps_of_f32(thk, ctx, H, Hkv, D, M, big, n_past):
+    rng = np.random.default_rng(M + D)
+    p, q, at = one_hot(rng, thk, ctx, H, Hkv, D, M, n_past, big)
+    mass = rng.random((Hkv, n_past + M)).astype(np.float32)
+    _, got = p.attend(q, n_past, mass, decode=M == 1)
+    exp, G = mass.astype(np.float64), H // Hkv
+    exp[:, at] += M * G
+    # a weight of exp2(0) times 1 / 1, or of 0; at most an addition for each row and head of the group, exact among whole numbers, and the last one
+    assert np.all(np.abs(got - exp) <= (M * G + 8) * EPS * exp), float(np.abs(got - exp).max())

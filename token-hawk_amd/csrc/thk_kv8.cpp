@@ -175,7 +175,10 @@ static int kv8_attention(thk_kv8* kv, const char* what, const float* q, int64_t 
             if (scored) { sp.scores = kv->scores; sp.scores_ld = (int64_t)a.c.n_blk * kKv8Block; }
             if (scored ? count_inside : inside && sp.n > 1) sp.counters = kv->counters;
             HIPCHK(ctx, launch_kv8_attn_split(a, sp, ctx->stream));
-        } else HIPCHK(ctx, launch_kv8_attn_tile(a, ctx->stream));
+        } else {
+            a.halves = true;
+            HIPCHK(ctx, launch_kv8_attn_tile(a, ctx->stream));
+        }
         if (mass_out && !scored) HIPCHK(ctx, launch_kv8_attn_mass(a, ctx->stream));
         mass_in = mass_out;
     }

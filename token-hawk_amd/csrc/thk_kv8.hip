@@ -991,9 +991,7 @@ __device__ __forceinline__ void split_f16(const float* x, float f, hf8& hi, hf8&
 }
 // The B operand of q for one column: parts of dimensions 64 (st / 2) + 16 (lane / 16) + 8 (st % 2) + j, st = 0 .. D/32 - 1.  Returns 1 / the power of two.
 template <int D>
-__device__ __forceinline__ float load_q_f16(const float* q, bool valid, hf8 (&hi)[D / 32], hf8 (&lo)[D / 32]) {
-    f4 x[D / 16];
-    load_q<D>(q, valid, x);
+__device__ __forceinline__ float q_f16(const f4 (&x)[D / 16], hf8 (&hi)[D / 32], hf8 (&lo)[D / 32]) {
     unsigned m = 0;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
@@ -1012,6 +1010,12 @@ __device__ __forceinline__ float load_q_f16(const float* q, bool valid, hf8 (&hi
         split_f16(y, up, hi[st], lo[st]);
     }
     return m >= 0x7F800000u ? as_f(0x7FC00000u) : ldexpf(1.f, e - 15);
+}
+// What turns the f16 sums of q and codes into scores.  Zero times a masked -inf would be NaN, so products below 2^-126 count as that: the sums
+// are below 2^30, a score moves by 2^-96 at most.
+__device__ __forceinline__ float score_factor(float qf, float ks) {
+    const float f = qf * ks;
+    return f < 0x1p-126f ? 0x1p-126f : f;
 }
 // consecutive logical indices on one XCD (workgroups are dealt to the 8 XCDs in turn): neighbours share a head's codes in that XCD's L2
 __device__ __forceinline__ int xcd_order(int id, int n) {
@@ -1068,7 +1072,9 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
         const int col = wcol0 + 16 * k + n;
         const bool valid = col < cols;
         lim[k] = valid ? a.n_past + col / G : T - 1;
-        qf[k] = load_q_f16<D>(a.q + (valid ? (size_t)(col / G) * c.H + hkv * G + col % G : 0) * D + ch * 16, valid, qh[k], ql[k]) * scale;
+        f4 x[D / 16];
+        load_q<D>(a.q + (valid ? (size_t)(col / G) * c.H + hkv * G + col % G : 0) * D + ch * 16, valid, x);
+        qf[k] = q_f16<D>(x, qh[k], ql[k]) * scale;
         m[k] = -INFINITY; l[k] = 0.f; ref[k] = kRefLeast;
 #pragma unroll
         for (int g = 0; g < NG; ++g) o[k][g] = f4{0.f, 0.f, 0.f, 0.f};
@@ -1125,9 +1131,7 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
             const bool edge = t * kKv8Tile + kKv8Tile - 1 > a.n_past + wrow0;
 #pragma unroll
             for (int k = 0; k < NC; ++k) {
-                // A block nobody sees has only -inf: its own factor may be NaN; and zero times -inf would be.  Products below 2^-126 count as
-                // that: the sums they scale are below 2^30, so a score moves by 2^-96 at most.
-                const float kq = qf[k] * ks, kf = pos > lim[k] ? 1.f : kq < 0x1p-126f ? 0x1p-126f : kq;
+                const float kf = pos > lim[k] ? 1.f : score_factor(qf[k], ks);      // a block nobody sees has only -inf: its own factor may be NaN
                 if (edge) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[k][i >> 2][i & 3] = pos + i <= lim[k] ? s[k][i >> 2][i & 3] : -INFINITY;
@@ -1235,12 +1239,14 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
 // ---------------------------------------------------------------- weight count of many rows
 // mass_out = mass_in + sum over the columns of exp2(s - m) / l.  A workgroup takes 64 positions; its W waves share the columns, 16 at a time
 // in turn, each with the K fragments of all 64 positions in registers and the next columns' q on the way; the waves' sums are added in a
-// fixed order.  Scores anew instead of kept ones: [rows][heads][positions] would be hundreds of times the cache.  512
+// fixed order.  Scores anew instead of kept ones: [rows][heads][positions] would be hundreds of times the cache.  They are computed as the attention
+// kernel computed them (F16: the one for many rows, its parts and order of products; else digits): m is one of them, and from any others large
+// scores' weights would be off by the exponential of the difference.  512
 // rows on 32 heads 13 us (15 in a trace), one workgroup a CU: its first tile's, with all rows' columns, has 1.8 times the mean to do and is what the
 // launch takes.  The vector instructions are 4.0 us of it on even load; waves wait 44 % of their cycles.
-template <int D, int W>
+template <int D, int W, bool F16>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_mass_tile_kernel(Kv8Attn a, float scale) {
-    constexpr int KC = D / 64;
+    constexpr int KC = D / 64, ST = D / 32;
     __shared__ float part[W][64];
     const Kv8View& c = a.c;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, ch = lane >> 4, hkv = blockIdx.y, G = c.H / c.Hkv, cols = a.M * G;
@@ -1253,6 +1259,13 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_mass_tile_kernel
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) kr[g][kc] = *reinterpret_cast<const i4*>(kb + 4 * g * D + kc * 64);
     const float ks = c.ks[(size_t)hkv * c.n_blk + (size_t)tile * 4 + ch];
+    hf8 kh[4][ST];
+    if (F16) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) { const HF8x2 h = codes_f16(kr[g][kc]); kh[g][2 * kc] = h.a; kh[g][2 * kc + 1] = h.b; }
+    }
     float sum[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum[i] = 0.f;
@@ -1269,23 +1282,36 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_mass_tile_kernel
 #pragma unroll 1
     for (; c0 < cols; c0 += 16 * W) {
         i4 qd[3][KC];
-        const float qf = q_digits<D>(x, qd) * scale, top = ml.x, inv = 1.f / ml.y;
+        hf8 qh[ST], ql[ST];
+        const float qf = (F16 ? q_f16<D>(x, qh, ql) : q_digits<D>(x, qd)) * scale, top = ml.x, inv = 1.f / ml.y;
         load(min(c0 + 16 * W, cols - 1));                                      // without a branch: the next ones, or any
         const int row = min(c0 + n, cols - 1) / G, lim = c0 + n < cols ? a.n_past + row : -1;
         const bool edge = __any(tile * kKv8Tile + kKv8Tile - 1 > lim);
-        const float kf = qf * ks;                                          // NaN at most in a block this column does not see: left out below
+        const float kf = F16 ? score_factor(qf, ks) : qf * ks;             // NaN at most in a block this column does not see: left out below
         float p[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            i4 acc[3];
+            f4 s;
+            if (F16) {
+                s = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int d = 0; d < 3; ++d) {
-                acc[d] = i4{0, 0, 0, 0};
+                for (int st = 0; st < ST; ++st) {
+                    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[g][st], qh[st], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[g][st], ql[st], s, 0, 0, 0);
+                }
+            } else {
+                i4 acc[3];
 #pragma unroll
-                for (int kc = 0; kc < KC; ++kc) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[g][kc], qd[d][kc], acc[d], 0, 0, 0);
+                for (int d = 0; d < 3; ++d) {
+                    acc[d] = i4{0, 0, 0, 0};
+#pragma unroll
+                    for (int kc = 0; kc < KC; ++kc) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[g][kc], qd[d][kc], acc[d], 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] = join_digits(acc[2][i], acc[1][i], acc[0][i]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[4 * g + i] = __builtin_amdgcn_exp2f(fmaf(join_digits(acc[2][i], acc[1][i], acc[0][i]), kf, -top));
+            for (int i = 0; i < 4; ++i) p[4 * g + i] = __builtin_amdgcn_exp2f(rounded_product(s[i], kf) - top);
         }
         if (edge) {                                                        // a row of NaN weights must not reach positions it does not see
 #pragma unroll
@@ -1404,7 +1430,10 @@ hipError_t launch_kv8_attn_tile(const Kv8Attn& a, hipStream_t st) {
 template <int D> static hipError_t mass_tile(const Kv8Attn& a, hipStream_t st) {
     const int tiles = (a.n_past + a.M + kKv8Tile - 1) / kKv8Tile;
     constexpr int W = D == 256 ? 4 : 8;
-    hipLaunchKernelGGL((kv8_mass_tile_kernel<D, W>), dim3(tiles, a.c.Hkv), dim3(64 * W), 0, st, a, kLog2e / sqrtf((float)D));
+    const dim3 grid(tiles, a.c.Hkv);
+    const float scale = kLog2e / sqrtf((float)D);
+    if (a.halves) hipLaunchKernelGGL((kv8_mass_tile_kernel<D, W, true>), grid, dim3(64 * W), 0, st, a, scale);
+    else hipLaunchKernelGGL((kv8_mass_tile_kernel<D, W, false>), grid, dim3(64 * W), 0, st, a, scale);
     const int rest = a.mass_n - (a.n_past + a.M);
     if (rest > 0 && a.mass_in != a.mass_out) hipLaunchKernelGGL(kv8_mass_rest_kernel, dim3((rest + 255) / 256, a.c.Hkv), dim3(256), 0, st, a);
     return hipGetLastError();

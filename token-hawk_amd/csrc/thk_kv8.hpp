@@ -37,6 +37,7 @@ struct Kv8Attn {
     float* out;                       // [M][H][D]
     int n_past, M;                    // row i sees positions <= n_past + i
     float2* ml;                       // [M][H] running maximum (base-2 scores) and sum of every row, for the weight count; or null
+    bool halves;                      // those are of scores from q in two f16 parts (the kernel for many rows), not from its digits
     const float* mass_in;             // [Hkv][mass_ld] or null (then no weights are counted)
     float* mass_out;
     int64_t mass_ld;
