@@ -959,7 +959,7 @@ __global__ __launch_bounds__(256) void kv8_attn_finish_kernel(Kv8Attn a, Kv8Spli
 //           only where the running maximum or ref moves, which a wave skips when none of its columns did.  For ref p counts
 //           as 2^-113 at least, so that v_scale * 2^(15 - ref) is finite: what the lo part then loses, 2^-151 of the scale, f32's own p does not hold.
 // Bound by the matrix instructions and, beside them, the softmax's vector ones (on f16 the two do not overlap): 2048 rows over 6144 positions, 32
-// heads on 8, 420 us, 481 GFLOP of f16 products (the f32 work twice) at 1.15 PFLOP/s; a large f16 matrix product reaches 1.16.
+// heads on 8, 424 - 430 us, 481 GFLOP of f16 products (the f32 work twice) at 1.13 PFLOP/s; a large f16 matrix product reaches 1.16.
 // S = 2: a second group of four waves takes every other tile, and its sums join the first's through LDS: 512 rows on 32 heads 18.8 -> 16.2 us.
 typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
@@ -1243,7 +1243,7 @@ __global__ __launch_bounds__(256 * S, 2) void kv8_attn_tile_kernel(Kv8Attn a, in
 // kernel computed them (F16: the one for many rows, its parts and order of products; else digits): m is one of them, and from any others large
 // scores' weights would be off by the exponential of the difference.  512
 // rows on 32 heads 13 us (15 in a trace), one workgroup a CU: its first tile's, with all rows' columns, has 1.8 times the mean to do and is what the
-// launch takes.  The vector instructions are 4.0 us of it on even load; waves wait 44 % of their cycles.
+// launch takes.  The vector instructions are 4.1 us of it on even load; waves wait 45 % of their cycles.
 template <int D, int W, bool F16>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv8_mass_tile_kernel(Kv8Attn a, float scale) {
     constexpr int KC = D / 64, ST = D / 32;
